@@ -385,6 +385,210 @@ void attn_prefill(const Tensor& q, const Tensor& cache, int64_t layer, const Ten
   vrm::paged_attention_prefill(a, cur_stream());
 }
 
+// ---------------------------------------------------------------- block-sparse decode
+int page_format(const Tensor& cache) { return is_q4_cache(cache) ? 2 : is_fp8_cache(cache) ? 1 : 0; }
+
+void check_rows16(const Tensor& t, const char* name) {
+  check_bf16_2d(t, name);
+  TORCH_CHECK(t.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, name,
+              ": rows must start on 16-byte boundaries");
+}
+
+// key bounds [pages, layers, KH, 2, D]: bf16, or e4m3 (of fp8 pages)
+void check_bounds(const Tensor& b, const char* op) {
+  TORCH_CHECK(b.is_cuda() && b.dim() == 5 && b.is_contiguous() && b.size(3) == 2, op,
+              ": key_bounds must be a contiguous [pages, layers, kv_heads, 2, head_dim] CUDA tensor");
+  TORCH_CHECK(b.scalar_type() == torch::kBFloat16 || b.scalar_type() == torch::kFloat8_e4m3fn, op,
+              ": key_bounds must be bf16 or fp8");
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(b.data_ptr()) % 16 == 0, op, ": key_bounds must be 16-byte aligned");
+}
+
+Tensor qk_norm_rope_kv_write(const Tensor& qkv, const OptT& wq, const OptT& wk, double eps, const OptT& positions,
+                             const OptT& cos_sin, Tensor& cache, const Tensor& slots, const OptT& kv_scale,
+                             int64_t layer, int64_t Hq, int64_t KH, int64_t D, const OptT& key_bounds,
+                             const OptT& out) {
+  const char* op = "qk_norm_rope_kv_write";
+  check_rows16(qkv, "qk_norm_rope_kv_write qkv");
+  TORCH_CHECK(Hq >= 1 && KH >= 1 && (D == 64 || D == 128), op, ": head_dim must be 64 or 128");
+  TORCH_CHECK(qkv.size(1) == (Hq + 2 * KH) * D, op, ": qkv width must be (Hq + 2 KH) * D");
+  check_cache(cache);
+  TORCH_CHECK(cache.size(3) == KH && cache_head_dim(cache) == D && cache.size(4) == 16, op,
+              ": cache kv_heads / head_dim / page size mismatch");
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(cache.data_ptr()) % 16 == 0, op, ": cache must be 16-byte aligned");
+  TORCH_CHECK(layer >= 0 && layer < cache.size(1), op, ": layer out of range");
+  const int64_t T = qkv.size(0);
+  TORCH_CHECK(slots.scalar_type() == torch::kInt32 && slots.is_contiguous() && slots.numel() >= T, op,
+              ": int32 slot_mapping [T]");
+  same_device(qkv, {&cache, &slots}, op);
+  same_device_opt(qkv, {&wq, &wk, &positions, &cos_sin, &kv_scale, &key_bounds, &out}, op);
+  TORCH_CHECK(has(wq) == has(wk), op, ": wq and wk go together");
+  vrm::AppendArgs a;
+  if (has(wq)) {
+    for (const OptT* w : {&wq, &wk})
+      TORCH_CHECK((*w)->scalar_type() == torch::kBFloat16 && (*w)->is_contiguous() && (*w)->numel() == D &&
+                      reinterpret_cast<uintptr_t>((*w)->data_ptr()) % 16 == 0,
+                  op, ": norm weights must be contiguous, 16-byte aligned bf16 [head_dim]");
+    a.wq = wq->data_ptr();
+    a.wk = wk->data_ptr();
+  }
+  a.eps = (float)eps;
+  if (has(cos_sin)) {
+    TORCH_CHECK(has(positions) && positions->scalar_type() == torch::kInt32 && positions->is_contiguous() &&
+                    positions->numel() >= T, op, ": int32 positions [T] required");
+    TORCH_CHECK(cos_sin->scalar_type() == torch::kFloat32 && cos_sin->is_contiguous() && cos_sin->dim() == 2 &&
+                    cos_sin->size(0) >= 1 && reinterpret_cast<uintptr_t>(cos_sin->data_ptr()) % 16 == 0,
+                op, ": cos_sin must be contiguous, 16-byte aligned fp32 [max_pos, rot_dim]");
+    TORCH_CHECK(cos_sin->size(1) <= D && cos_sin->size(1) % 2 == 0, op, ": rot_dim");
+    a.positions = positions->data_ptr<int>();
+    a.cos_sin = cos_sin->data_ptr<float>();
+    a.rot_dim = (int)cos_sin->size(1);
+    a.max_pos = (int)cos_sin->size(0);
+  }
+  a.fmt = page_format(cache);
+  if (a.fmt == 1) {
+    TORCH_CHECK(has(kv_scale) && kv_scale->scalar_type() == torch::kFloat32 && kv_scale->is_contiguous() &&
+                    kv_scale->numel() == cache.size(1) * 2 * KH,
+                op, ": fp8 pages need kv_scale fp32 [layers, 2, kv_heads]");
+    a.kv_scale = kv_scale->data_ptr<float>();
+  }
+  if (has(key_bounds)) {
+    check_bounds(*key_bounds, op);
+    TORCH_CHECK(key_bounds->size(0) == cache.size(0) && key_bounds->size(1) == cache.size(1) &&
+                    key_bounds->size(2) == KH && key_bounds->size(4) == D, op, ": key_bounds do not match the cache");
+    TORCH_CHECK((key_bounds->scalar_type() == torch::kFloat8_e4m3fn) == (a.fmt == 1), op,
+                ": key_bounds are fp8 for fp8 pages, else bf16");
+    a.bounds = key_bounds->data_ptr();
+  }
+  const c10::cuda::CUDAGuard guard(qkv.device());
+  Tensor q = has(out) ? *out : torch::empty({T, Hq * D}, qkv.options());
+  check_rows16(q, "qk_norm_rope_kv_write out");
+  TORCH_CHECK(q.size(0) >= T && q.size(1) >= Hq * D, op, ": out must be [T, Hq * D]");
+  if (has(out) && q.is_alias_of(qkv)) {
+    // the q columns of qkv itself, or columns that no head of qkv lies in
+    const int64_t gap = q.storage_offset() - qkv.storage_offset();
+    TORCH_CHECK(q.stride(0) == qkv.stride(0) && (gap == 0 || (gap >= qkv.size(1) && gap + Hq * D <= qkv.stride(0))),
+                op, ": out overlaps qkv");
+  }
+  a.qkv = qkv.data_ptr();
+  a.ld_qkv = qkv.stride(0);
+  a.T = (int)T;
+  a.Hq = (int)Hq;
+  a.KH = (int)KH;
+  a.D = (int)D;
+  a.cache = cache.data_ptr();
+  a.num_layers = (int)cache.size(1);
+  a.layer = (int)layer;
+  a.num_pages = cache.size(0);
+  a.slots = slots.data_ptr<int>();
+  a.q_out = q.data_ptr();
+  a.ld_out = q.stride(0);
+  vrm::qk_norm_rope_kv_write(a, cur_stream());
+  return q;
+}
+
+// The row -> sequence metadata that select_pages and paged_attention_selected share.
+template <typename Args>
+void set_rows(Args& a, const Tensor& q, const Tensor& block_tables, const Tensor& context_lens, const OptT& cu_q,
+              int64_t Hq, int64_t KH, int64_t D, const char* op) {
+  check_rows16(q, op);
+  TORCH_CHECK(KH >= 1 && Hq >= 1 && Hq % KH == 0 && Hq / KH <= 8, op, ": GQA group must be <= 8 heads");
+  TORCH_CHECK(D == 64 || D == 128, op, ": head_dim must be 64 or 128");
+  TORCH_CHECK(q.size(1) >= Hq * D, op, ": q must be [T, >= Hq * D]");
+  TORCH_CHECK(block_tables.scalar_type() == torch::kInt32 && block_tables.dim() == 2 && block_tables.stride(1) == 1,
+              op, ": block_tables must be int32 [B, max_pages]");
+  TORCH_CHECK(context_lens.scalar_type() == torch::kInt32 && context_lens.is_contiguous(), op, ": int32 context_lens");
+  same_device(q, {&block_tables, &context_lens}, op);
+  same_device_opt(q, {&cu_q}, op);
+  int64_t B = q.size(0);
+  if (has(cu_q)) {
+    TORCH_CHECK(cu_q->scalar_type() == torch::kInt32 && cu_q->is_contiguous() && cu_q->numel() >= 1, op,
+                ": int32 cu_q [B + 1]");
+    B = cu_q->numel() - 1;
+    a.cu_q = cu_q->data_ptr<int>();
+  }
+  TORCH_CHECK(block_tables.size(0) >= B && context_lens.numel() >= B, op, ": batch sizes");
+  a.q = q.data_ptr();
+  a.ld_q = q.stride(0);
+  a.T = (int)q.size(0);
+  a.B = (int)B;
+  a.KH = (int)KH;
+  a.G = (int)(Hq / KH);
+  a.D = (int)D;
+  a.block_tables = block_tables.data_ptr<int>();
+  a.bt_stride = (int)block_tables.stride(0);
+  a.max_pages = (int)block_tables.size(1);
+  a.context_lens = context_lens.data_ptr<int>();
+}
+
+Tensor select_pages(const Tensor& q, const Tensor& key_bounds, int64_t layer, const Tensor& block_tables,
+                    const Tensor& context_lens, int64_t Hq, int64_t budget, int64_t sinks, int64_t recent,
+                    const OptT& cu_q, const OptT& out) {
+  const char* op = "select_pages";
+  check_bounds(key_bounds, op);
+  TORCH_CHECK(layer >= 0 && layer < key_bounds.size(1), op, ": layer out of range");
+  TORCH_CHECK(sinks >= 0 && recent >= 1 && budget >= sinks + recent && budget <= INT32_MAX, op,
+              ": needs sinks >= 0, recent >= 1 and budget >= sinks + recent");
+  vrm::SelectArgs a;
+  set_rows(a, q, block_tables, context_lens, cu_q, Hq, key_bounds.size(2), key_bounds.size(4), op);
+  same_device(q, {&key_bounds}, op);
+  same_device_opt(q, {&out}, op);
+  const c10::cuda::CUDAGuard guard(q.device());
+  Tensor pages = has(out) ? *out : torch::empty({q.size(0), a.KH, budget}, block_tables.options());
+  TORCH_CHECK(pages.scalar_type() == torch::kInt32 && pages.is_contiguous() && pages.dim() == 3 &&
+                  pages.size(0) >= q.size(0) && pages.size(1) == a.KH && pages.size(2) == budget,
+              op, ": out must be contiguous int32 [T, kv_heads, budget]");
+  a.bounds = key_bounds.data_ptr();
+  a.f8 = key_bounds.scalar_type() == torch::kFloat8_e4m3fn;
+  a.num_layers = (int)key_bounds.size(1);
+  a.layer = (int)layer;
+  a.num_pages = key_bounds.size(0);
+  a.budget = (int)budget;
+  a.sinks = (int)sinks;
+  a.recent = (int)recent;
+  a.out = pages.data_ptr<int>();
+  vrm::select_pages(a, cur_stream());
+  return pages;
+}
+
+Tensor attn_selected(const Tensor& q, const Tensor& cache, int64_t layer, const Tensor& block_tables,
+                     const Tensor& context_lens, const Tensor& pages, const OptT& kv_scale, double sm_scale,
+                     int64_t Hq, const OptT& cu_q, const OptT& out) {
+  const char* op = "paged_attention_selected";
+  check_cache(cache);
+  TORCH_CHECK(cache.size(4) == 16 && reinterpret_cast<uintptr_t>(cache.data_ptr()) % 16 == 0, op,
+              ": cache must be 16-byte aligned with pages of 16 tokens");
+  TORCH_CHECK(layer >= 0 && layer < cache.size(1), op, ": layer out of range");
+  vrm::AttendArgs a;
+  set_rows(a, q, block_tables, context_lens, cu_q, Hq, cache.size(3), cache_head_dim(cache), op);
+  TORCH_CHECK(pages.scalar_type() == torch::kInt32 && pages.is_contiguous() && pages.dim() == 3 &&
+                  pages.size(0) >= q.size(0) && pages.size(1) == a.KH,
+              op, ": pages must be contiguous int32 [T, kv_heads, n]");
+  same_device(q, {&cache, &pages}, op);
+  same_device_opt(q, {&kv_scale, &out}, op);
+  a.fmt = page_format(cache);
+  if (a.fmt == 1) {
+    TORCH_CHECK(has(kv_scale) && kv_scale->scalar_type() == torch::kFloat32 && kv_scale->is_contiguous() &&
+                    kv_scale->numel() == cache.size(1) * 2 * cache.size(3),
+                op, ": fp8 pages need kv_scale fp32 [layers, 2, kv_heads]");
+    a.kv_scale = kv_scale->data_ptr<float>();
+  }
+  const c10::cuda::CUDAGuard guard(q.device());
+  Tensor o = has(out) ? *out : torch::empty({q.size(0), Hq * a.D}, q.options());
+  check_rows16(o, "paged_attention_selected out");
+  TORCH_CHECK(o.size(0) >= q.size(0) && o.size(1) >= Hq * a.D, op, ": out must be [T, Hq * D]");
+  a.cache = cache.data_ptr();
+  a.num_layers = (int)cache.size(1);
+  a.layer = (int)layer;
+  a.num_pages = cache.size(0);
+  a.pages = pages.data_ptr<int>();
+  a.S = (int)pages.size(2);
+  a.sm_scale = (float)sm_scale;
+  a.out = o.data_ptr();
+  a.ld_o = o.stride(0);
+  vrm::paged_attention_selected(a, cur_stream());
+  return o;
+}
+
 // ---------------------------------------------------------------- sampling
 void argmax(const Tensor& logits, Tensor& out) {
   check_bf16_2d(logits, "argmax logits");
@@ -1262,6 +1466,16 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("paged_attention_prefill", &attn_prefill, py::arg("q"), py::arg("cache"), py::arg("layer"),
         py::arg("block_tables"), py::arg("cu_q"), py::arg("context_lens"), py::arg("kv_scale"), py::arg("sm_scale"),
         py::arg("out"), py::arg("max_q_len"), py::arg("num_q_heads"));
+  m.def("qk_norm_rope_kv_write", &qk_norm_rope_kv_write, py::arg("qkv"), py::arg("wq"), py::arg("wk"), py::arg("eps"),
+        py::arg("positions"), py::arg("cos_sin"), py::arg("cache"), py::arg("slot_mapping"), py::arg("kv_scale"),
+        py::arg("layer"), py::arg("num_q_heads"), py::arg("num_kv_heads"), py::arg("head_dim"), py::arg("key_bounds"),
+        py::arg("out"));
+  m.def("select_pages", &select_pages, py::arg("q"), py::arg("key_bounds"), py::arg("layer"), py::arg("block_tables"),
+        py::arg("context_lens"), py::arg("num_q_heads"), py::arg("budget"), py::arg("sinks"), py::arg("recent"),
+        py::arg("cu_q"), py::arg("out"));
+  m.def("paged_attention_selected", &attn_selected, py::arg("q"), py::arg("cache"), py::arg("layer"),
+        py::arg("block_tables"), py::arg("context_lens"), py::arg("pages"), py::arg("kv_scale"), py::arg("sm_scale"),
+        py::arg("num_q_heads"), py::arg("cu_q"), py::arg("out"));
   m.def("decode_attention_splits", [](int64_t B, int64_t KH, int64_t max_pages) {
     return vrm::decode_attention_choose_splits((int)B, (int)KH, (int)max_pages);
   });

@@ -425,6 +425,73 @@ void paged_attention_prefill(const PrefillAttnArgs& a, cudaStream_t stream);
 // Selects the tcgen05 prefill kernel for bf16 pages (default off, VRM_PREFILL_TC=1 on).
 void set_prefill_tc(bool on);
 
+// ---------------------------------------------------------------- block-sparse decode (sparse_kv.cu)
+// Page formats of `fmt`: 0 bf16, 1 fp8 e4m3 (kv_scale), 2 four-bit rows (vrm_common.cuh).
+// Key bounds [pages, layers, KH, {min, max}, D]: bf16, or e4m3 codes beside fp8 pages.
+struct AppendArgs {
+  const void* qkv = nullptr;           // bf16 [T, (Hq + 2 KH) * D]
+  int64_t ld_qkv = 0;
+  const void* wq = nullptr;            // bf16 [D] RMSNorm weights of the q / k heads (null: none)
+  const void* wk = nullptr;
+  float eps = 0.f;
+  int T = 0, Hq = 0, KH = 0, D = 0;
+  const int* positions = nullptr;      // [T] (rot_dim > 0)
+  const float* cos_sin = nullptr;      // [max_pos, rot_dim] = [cos | sin]
+  int rot_dim = 0, max_pos = 0;
+  void* cache = nullptr;
+  int fmt = 0, num_layers = 0, layer = 0;
+  int64_t num_pages = 0;
+  const int* slots = nullptr;          // [T] page * 16 + offset, < 0: the token is not stored
+  const float* kv_scale = nullptr;     // [layers, 2, KH] (fp8 pages)
+  void* bounds = nullptr;              // key bounds, or null
+  void* q_out = nullptr;               // bf16, token t head h at q_out + t * ld_out + h * D
+  int64_t ld_out = 0;
+  int heads_per_group = 0, q_groups = 0, v_groups = 0;   // set by the launcher
+  uint32_t* err = nullptr;             // error word (set by the launcher)
+};
+void qk_norm_rope_kv_write(const AppendArgs& a, cudaStream_t stream);
+
+// Query row t belongs to sequence t, or with cu_q [B + 1] rows cu_q[b] .. cu_q[b + 1] - 1
+// are the last tokens of sequence b; rows behind cu_q[B] are left alone.
+struct SelectArgs {
+  const void* q = nullptr;             // bf16, row t head h at q + t * ld_q + h * D
+  int64_t ld_q = 0;
+  int T = 0, B = 0, KH = 0, G = 0, D = 0;
+  const void* bounds = nullptr;
+  bool f8 = false;                     // bounds are e4m3 codes
+  int num_layers = 0, layer = 0;
+  int64_t num_pages = 0;
+  const int* block_tables = nullptr;   // [B, bt_stride], max_pages columns used
+  int bt_stride = 0, max_pages = 0;
+  const int* context_lens = nullptr;   // [B]
+  const int* cu_q = nullptr;
+  int budget = 0, sinks = 0, recent = 0;
+  int* out = nullptr;                  // [T, KH, budget] ascending page indexes, -1 behind the last
+  uint32_t* err = nullptr;
+};
+void select_pages(const SelectArgs& a, cudaStream_t stream);
+
+struct AttendArgs {
+  const void* q = nullptr;
+  int64_t ld_q = 0;
+  int T = 0, B = 0, KH = 0, G = 0, D = 0;
+  const void* cache = nullptr;
+  int fmt = 0, num_layers = 0, layer = 0;
+  int64_t num_pages = 0;
+  const int* block_tables = nullptr;
+  int bt_stride = 0, max_pages = 0;
+  const int* context_lens = nullptr;
+  const int* cu_q = nullptr;
+  const int* pages = nullptr;          // [T, KH, S]
+  int S = 0;
+  const float* kv_scale = nullptr;
+  float sm_scale = 1.f;
+  void* out = nullptr;                 // bf16, row t head h at out + t * ld_o + h * D
+  int64_t ld_o = 0;
+  uint32_t* err = nullptr;
+};
+void paged_attention_selected(const AttendArgs& a, cudaStream_t stream);
+
 // ---------------------------------------------------------------- sampling (sampling.cu)
 void argmax_rows(const void* logits, int64_t ld, int B, int V, int* out, cudaStream_t stream);
 void sample_rows(const void* logits, int64_t ld, int B, int V, const float* temperature, const int* top_k,

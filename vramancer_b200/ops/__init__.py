@@ -440,6 +440,197 @@ def paged_attention_prefill(q: torch.Tensor, cache: torch.Tensor, layer: int, bl
     return out
 
 
+# --------------------------------------------------------------------------- block-sparse decode
+def key_bounds_for(cache: torch.Tensor) -> torch.Tensor:
+    """Zeroed key bounds for a KV pool [pages, layers, 2, KH, 16, row]: [pages, layers, KH, 2, D]
+    (minimum, maximum), bf16, or e4m3 codes (values before kv_scale) for fp8 pools."""
+    D = cache_head_dim(cache)
+    dt = torch.float8_e4m3fn if cache.dtype == torch.float8_e4m3fn else torch.bfloat16
+    return torch.zeros(cache.shape[0], cache.shape[1], cache.shape[3], 2, D, dtype=dt, device=cache.device)
+
+
+def qk_norm_rope_kv_write(qkv: torch.Tensor, wq: Optional[torch.Tensor], wk: Optional[torch.Tensor], eps: float,
+                          positions: Optional[torch.Tensor], cos_sin: Optional[torch.Tensor], cache: torch.Tensor,
+                          slot_mapping: torch.Tensor, kv_scale: Optional[torch.Tensor], layer: int, num_q_heads: int,
+                          num_kv_heads: int, head_dim: int, *, key_bounds: Optional[torch.Tensor] = None,
+                          out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """`qk_rmsnorm` (with wq / wk), `rope_kv_write` and the key bounds of the written pages in
+    one pass over qkv [T, (Hq + 2 KH) * D]; returns the q heads [T, Hq * D] (qkv is left as it
+    is; `out` may be its q columns).  Values stay fp32 from the norm to the one rounding of q
+    to bf16 and of k / v to the page format.
+
+    With `key_bounds` (`key_bounds_for`) every page that is written gets the elementwise
+    minimum and maximum of its stored keys, from its first row to the last row written here
+    (rows behind are not part of the sequence).  For that the tokens of a page must be
+    adjacent in the batch and in the order of their slots, as the tokens of a prefill chunk, a
+    verify step and a decode batch are.  Infinite keys count as the largest finite value of
+    the bounds' type, a NaN as both its extremes.  Slots must be distinct; a slot < 0 is not
+    stored."""
+    if qkv.is_cuda:
+        return native().qk_norm_rope_kv_write(qkv, wq, wk, eps, positions, cos_sin, cache, slot_mapping, kv_scale,
+                                              layer, num_q_heads, num_kv_heads, head_dim, key_bounds, out)
+    T = qkv.shape[0]
+    Hq, KH, D = num_q_heads, num_kv_heads, head_dim
+    if (wq is None) != (wk is None):
+        raise ValueError("qk_norm_rope_kv_write: wq and wk go together")
+    x = qkv.view(T, Hq + 2 * KH, D).float()
+    qk, v = x[:, :Hq + KH].clone(), x[:, Hq + KH:]
+    if wq is not None:
+        w = torch.cat([wq.float().expand(Hq, D), wk.float().expand(KH, D)])
+        qk = qk * torch.rsqrt(qk.pow(2).mean(-1, keepdim=True) + eps) * w
+    if cos_sin is not None and T > 0:
+        rot = cos_sin.shape[1]
+        half = rot // 2
+        cs = cos_sin[positions[:T].long()]
+        c, s = cs[:, None, :half], cs[:, None, half:]
+        x1, x2 = qk[..., :half].clone(), qk[..., half:rot].clone()
+        qk[..., :half] = x1 * c - x2 * s
+        qk[..., half:rot] = x2 * c + x1 * s
+    q = qk[:, :Hq].reshape(T, Hq * D).to(qkv.dtype)
+    if out is None:
+        out = q
+    else:
+        out[:T, :Hq * D] = q
+    slots = slot_mapping[:T].long()
+    idx = torch.nonzero(slots >= 0).flatten()
+    if idx.numel() == 0:
+        return out
+    page, off = slots[idx] // 16, slots[idx] % 16
+    kv = torch.stack([qk[idx, Hq:], v[idx]], 1)                     # [n, 2, KH, D]
+    if cache.dtype == torch.uint8:
+        from ..kv import q4
+        kv = q4.quantize(kv)
+    elif cache.dtype == torch.float8_e4m3fn:
+        kv = (kv / kv_scale[layer].view(1, 2, KH, 1)).clamp(-448, 448).to(cache.dtype)
+    else:
+        kv = kv.to(cache.dtype)
+    for n in range(idx.numel()):
+        cache[page[n], layer, :, :, off[n]] = kv[n]
+    if key_bounds is not None:
+        top = torch.finfo(key_bounds.dtype).max
+        for p in page.unique().tolist():
+            rows = cache[p, layer, 0, :, : int(off[page == p].max()) + 1]
+            if cache.dtype == torch.uint8:
+                from ..kv import q4
+                rows = q4.dequantize(rows)
+            rows = rows.float()
+            nan = rows.isnan()
+            key_bounds[p, layer, :, 0] = rows.masked_fill(nan, -top).amin(1).clamp(-top, top).to(key_bounds.dtype)
+            key_bounds[p, layer, :, 1] = rows.masked_fill(nan, top).amax(1).clamp(-top, top).to(key_bounds.dtype)
+    return out
+
+
+def _query_rows(T: int, context_lens: torch.Tensor, cu_q: Optional[torch.Tensor]):
+    """(row, sequence, tokens the row sees) of the query rows of block-sparse attention."""
+    if cu_q is None:
+        return [(t, t, max(0, int(context_lens[t]))) for t in range(T)]
+    rows = []
+    for b in range(cu_q.numel() - 1):
+        s0, s1 = int(cu_q[b]), int(cu_q[b + 1])
+        rows += [(t, b, max(0, int(context_lens[b]) - (s1 - 1 - t))) for t in range(s0, min(s1, T))]
+    return rows
+
+
+def _bound_values(b: torch.Tensor) -> torch.Tensor:
+    """Key bounds in 64 bits, every code read as a finite value: a bf16 infinity or NaN as
+    2^128 times its significand, the e4m3 NaN code as 480."""
+    if b.dtype == torch.float8_e4m3fn:
+        u = b.contiguous().view(torch.uint8).long()
+        e, m, bias, bits = (u >> 3) & 15, u & 7, 7, 3
+        neg = (u >> 7) > 0
+    else:
+        u = b.contiguous().view(torch.int16).long() & 0xFFFF
+        e, m, bias, bits = (u >> 7) & 255, u & 127, 127, 7
+        neg = (u >> 15) > 0
+    frac = m.double() / 2 ** bits + (e > 0).double()
+    val = torch.ldexp(frac, (e.clamp(min=1) - bias).double())
+    return torch.where(neg, -val, val)
+
+
+def select_pages(q: torch.Tensor, key_bounds: torch.Tensor, layer: int, block_tables: torch.Tensor,
+                 context_lens: torch.Tensor, num_q_heads: int, budget: int, *, sinks: int = 1, recent: int = 1,
+                 cu_q: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The pages each query row reads: int32 [T, KH, budget] indexes into the row's block
+    table, ascending, -1 behind the last.
+
+    q [T, >= Hq * D] holds rotated query rows, one per sequence, or with `cu_q` [B + 1] rows
+    cu_q[b] .. cu_q[b + 1] - 1 as the last tokens of sequence b (context_lens count them);
+    rows behind cu_q[B] are left as they were.  A row that sees at most `budget` pages gets
+    all of them.  Otherwise it gets the first `sinks`, the last `recent` (the page that is
+    being filled among them: its bounds are not used) and of the others those with the
+    largest
+
+        sum_d ( sum_g max(q_gd, 0) * max_d  +  sum_g min(q_gd, 0) * min_d ),
+
+    g over the query heads of the kv head: no key of the page gives the group a larger sum of
+    scores.  Scores are compared in 64 bits; ties go to the lowest page, a NaN comes first."""
+    if q.is_cuda:
+        return native().select_pages(q, key_bounds, layer, block_tables, context_lens, num_q_heads, budget, sinks,
+                                     recent, cu_q, out)
+    if sinks < 0 or recent < 1 or budget < sinks + recent:
+        raise ValueError("select_pages: needs sinks >= 0, recent >= 1 and budget >= sinks + recent")
+    T = q.shape[0]
+    KH, D = key_bounds.shape[2], key_bounds.shape[4]
+    G = num_q_heads // KH
+    if out is None:
+        out = torch.full((T, KH, budget), -1, dtype=torch.int32)
+    for t, b, n in _query_rows(T, context_lens, cu_q):
+        total = min((n + 15) // 16, block_tables.shape[1])
+        out[t] = -1
+        if total <= budget:
+            out[t, :, :total] = torch.arange(total, dtype=torch.int32)
+            continue
+        qd = q[t, : num_q_heads * D].double().view(KH, G, D)
+        up = torch.where(qd >= 0, qd, 0.0).sum(1)
+        dn = torch.where(qd >= 0, 0.0, qd).sum(1)
+        bd = _bound_values(key_bounds[block_tables[b, :total].long(), layer])     # [P, KH, 2, D]
+        s = (up * bd[:, :, 1] + dn * bd[:, :, 0]).sum(-1).t()                     # [KH, P]
+        s = torch.where(s.isnan(), math.inf, s)
+        mid = s[:, sinks: total - recent]
+        need = budget - sinks - recent
+        for h in range(KH):
+            # a NaN outranks an infinity; stable sort: ties to the lowest page
+            nan = (up[h] * bd[sinks: total - recent, h, 1] + dn[h] * bd[sinks: total - recent, h, 0]).sum(-1).isnan()
+            order = torch.sort(mid[h], descending=True, stable=True).indices
+            order = torch.cat([order[nan[order]], order[~nan[order]]])[:need]
+            out[t, h] = torch.cat([torch.arange(sinks), order.sort().values + sinks,
+                                   torch.arange(total - recent, total)]).to(torch.int32)
+    return out
+
+
+def paged_attention_selected(q: torch.Tensor, cache: torch.Tensor, layer: int, block_tables: torch.Tensor,
+                             context_lens: torch.Tensor, pages: torch.Tensor, kv_scale: Optional[torch.Tensor],
+                             sm_scale: float, num_q_heads: int, *, cu_q: Optional[torch.Tensor] = None,
+                             out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of query rows (laid out as in `select_pages`) over the tokens of the listed
+    pages only: pages int32 [T, KH, n] holds indexes into the row's block table, -1 (or any
+    page behind the row's context) for none.  Tokens behind the row's own are never read.  A
+    row without pages gives zeros; rows behind cu_q[B] are left as they were."""
+    if q.is_cuda:
+        return native().paged_attention_selected(q, cache, layer, block_tables, context_lens, pages, kv_scale,
+                                                 sm_scale, num_q_heads, cu_q, out)
+    T = q.shape[0]
+    D = cache_head_dim(cache)
+    KH = cache.shape[3]
+    G = num_q_heads // KH
+    if out is None:
+        out = torch.zeros(T, num_q_heads * D, dtype=q.dtype)
+    for t, b, n in _query_rows(T, context_lens, cu_q):
+        o = out[t, : num_q_heads * D].view(KH, G, D)
+        total = min((n + 15) // 16, block_tables.shape[1])
+        for h in range(KH):
+            sel = [p for p in pages[t, h].tolist() if 0 <= p < total]
+            if not sel:
+                o[h] = 0
+                continue
+            k, v = _gather_kv(cache, layer, block_tables[b].long()[sel], 16 * len(sel), kv_scale)
+            tok = (torch.tensor(sel)[:, None] * 16 + torch.arange(16)).flatten()
+            k, v = k[tok < n, h], v[tok < n, h]
+            s = q[t, h * G * D: (h + 1) * G * D].float().view(G, D) @ k.t() * sm_scale
+            o[h] = (torch.softmax(s, dim=-1) @ v).to(out.dtype)
+    return out
+
+
 # --------------------------------------------------------------------------- elementwise
 def silu_mul(x: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """[T, 2I] (gate | up) -> silu(gate) * up."""
