@@ -13,7 +13,6 @@
 
 #include <algorithm>
 #include <climits>
-#include <cstdlib>
 #include <type_traits>
 
 #include "vrm_common.cuh"
@@ -26,28 +25,38 @@ namespace {
 
 constexpr int kPageTok = 16;
 
-// 16-byte / 8-byte / 4-byte loads that do not allocate in L1 (every byte is used once)
-__device__ __forceinline__ uint4 ld_stream16(const void* p) {
-  uint4 v;
-  asm volatile("ld.global.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
-  return v;
-}
-__device__ __forceinline__ uint2 ld_stream8(const void* p) {
-  uint2 v;
-  asm volatile("ld.global.L1::no_allocate.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-  return v;
-}
-__device__ __forceinline__ uint32_t ld_stream4(const void* p) {
-  uint32_t v;
-  asm volatile("ld.global.L1::no_allocate.b32 %0, [%1];" : "=r"(v) : "l"(p));
-  return v;
+// 4, 8 or 16 bytes that are used once: not kept in L1.  Volatile: loads stay where they are
+// written, ahead of the arithmetic that hides their latency.
+template <int N>
+__device__ __forceinline__ void ld_stream(uint32_t* v, const void* p) {
+  if constexpr (N == 16)
+    asm volatile("ld.global.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+                 : "l"(p));
+  else if constexpr (N == 8)
+    asm volatile("ld.global.L1::no_allocate.v2.b32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "l"(p));
+  else
+    asm volatile("ld.global.L1::no_allocate.b32 %0, [%1];" : "=r"(v[0]) : "l"(p));
 }
 
-__device__ __forceinline__ float fp8_to_f32(uint32_t code) {
-  __half_raw h = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)code, __NV_E4M3);
-  return __half2float(*reinterpret_cast<__half*>(&h));
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// the e4m3 pair in the low half of v (exact)
+__device__ __forceinline__ uint32_t fp8x2_to_half2(uint32_t v) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)v));
+  return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
 }
 
 // The sequence of query row t and the tokens the row sees.  Without cu_q rows are
@@ -87,9 +96,9 @@ __device__ __forceinline__ bool find_row(int t, const int* cu_q, const int* cont
 // Rows are handled by D / 16 lanes, 16 dims each: dims [8j, 8j + 8) and the same of the
 // other half of the head, so that with a rotation over the whole head both dims of every
 // rotated pair sit in one lane; a 128-thread block takes kRows rows at a time.
-// blockIdx.x is a tile of kRows tokens, blockIdx.y a group of q heads, v heads or one k
-// head.  With key bounds a k block owns the runs (maximal sequences of adjacent tokens in
-// consecutive slots of one page) that begin in its tile, wherever they end, so every
+// A block takes a group of q heads or of v heads of a tile of kRows tokens, or one k head of
+// a k tile.  With key bounds a k block owns the runs (maximal sequences of adjacent tokens
+// in consecutive slots of one page) that begin in its tile, wherever they end, so every
 // page's bounds have one writer and do not depend on the order of the blocks.
 template <int D>
 struct AppendShape {
@@ -102,8 +111,8 @@ enum : int { kRotNone = 0, kRotFull = 1, kRotPart = 2 };
 
 // x (16 dims of a row per lane) -> RMSNorm with weight w (null: none), then the rotation
 template <int D, int ROT>
-__device__ __forceinline__ void norm_rotate(float (&x)[16], const __nv_bfloat16* w, float eps, int j, const float* cs,
-                                            int rot_dim, float* scratch) {
+__device__ __forceinline__ void norm_rotate(float (&x)[16], const __nv_bfloat16* w, float eps, int j,
+                                            const float (&cs)[16], const float* cs_row, int rot_dim, float* scratch) {
   constexpr int kLanes = AppendShape<D>::kLanes;
   if (w != nullptr) {
     float ss = 0.f;
@@ -123,14 +132,7 @@ __device__ __forceinline__ void norm_rotate(float (&x)[16], const __nv_bfloat16*
   }
   if constexpr (ROT == kRotFull) {
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      const float4 c = *reinterpret_cast<const float4*>(cs + 8 * j + 4 * q);
-      const float4 s = *reinterpret_cast<const float4*>(cs + D / 2 + 8 * j + 4 * q);
-      rope_rotate(x[4 * q], x[8 + 4 * q], c.x, s.x, x[4 * q], x[8 + 4 * q]);
-      rope_rotate(x[4 * q + 1], x[9 + 4 * q], c.y, s.y, x[4 * q + 1], x[9 + 4 * q]);
-      rope_rotate(x[4 * q + 2], x[10 + 4 * q], c.z, s.z, x[4 * q + 2], x[10 + 4 * q]);
-      rope_rotate(x[4 * q + 3], x[11 + 4 * q], c.w, s.w, x[4 * q + 3], x[11 + 4 * q]);
-    }
+    for (int i = 0; i < 8; ++i) rope_rotate(x[i], x[8 + i], cs[i], cs[8 + i], x[i], x[8 + i]);
   } else if constexpr (ROT == kRotPart) {
     // the partner of a dim sits in another lane: exchange through the row's scratch
 #pragma unroll
@@ -142,10 +144,10 @@ __device__ __forceinline__ void norm_rotate(float (&x)[16], const __nv_bfloat16*
       const int d = (i < 8 ? 0 : D / 2 - 8) + 8 * j + i;
       float a, b;
       if (d < half) {
-        rope_rotate(x[i], scratch[d + half], cs[d], cs[half + d], a, b);
+        rope_rotate(x[i], scratch[d + half], cs_row[d], cs_row[half + d], a, b);
         x[i] = a;
       } else if (d < rot_dim) {
-        rope_rotate(scratch[d - half], x[i], cs[d - half], cs[d], a, b);
+        rope_rotate(scratch[d - half], x[i], cs_row[d - half], cs_row[d], a, b);
         x[i] = b;
       }
     }
@@ -166,35 +168,42 @@ __device__ __forceinline__ void unpack8(uint4 v, float* x) {
 __device__ __forceinline__ uint4 pack8(const float* x) {
   return make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
 }
+// four e4m3 codes -> 2 x f16x2 (exact)
+__device__ __forceinline__ uint2 fp8x4_to_half4(uint32_t v) {
+  return make_uint2(fp8x2_to_half2(v), fp8x2_to_half2(v >> 16));
+}
 
-// One rounding from fp32 to the page format; x becomes the value that readers of the row
-// see (fp8: the e4m3 code, before the head's scale).  dst: the stored row; `on`: this
-// lane's row is stored (all lanes take part in the shuffles).
+// One rounding from fp32 to the page format.  dst: the stored row; `on`: this lane's row is
+// stored (all lanes take part in the shuffles).  key: the 16 stored values in the 16-bit
+// type the bounds are compared in: f16 for fp8 codes, else bf16 (four-bit values are rounded
+// to the bounds' type here; rounding is monotone, so it commutes with min and max).
 template <int D, int FMT>
-__device__ __forceinline__ void store_kv_row(uint8_t* dst, float (&x)[16], float scale, int j, bool on) {
+__device__ __forceinline__ void store_kv_row(uint8_t* dst, const float (&x)[16], float scale, int j, bool on,
+                                             uint4 (&key)[2]) {
   if constexpr (FMT == kFmtBf16) {
-    const uint4 a = pack8(x), b = pack8(x + 8);
+    key[0] = pack8(x);
+    key[1] = pack8(x + 8);
     if (on) {
-      *reinterpret_cast<uint4*>(dst + 16 * j) = a;
-      *reinterpret_cast<uint4*>(dst + D + 16 * j) = b;
+      *reinterpret_cast<uint4*>(dst + 16 * j) = key[0];
+      *reinterpret_cast<uint4*>(dst + D + 16 * j) = key[1];
     }
-    unpack8(a, x);
-    unpack8(b, x + 8);
   } else if constexpr (FMT == kFmtFp8) {
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      w[i] = 0;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const uint32_t q = __nv_cvt_float_to_fp8(__fdiv_rn(x[4 * i + k], scale), __NV_SATFINITE, __NV_E4M3);
-        w[i] |= q << (8 * k);
-        x[4 * i + k] = fp8_to_f32(q);
-      }
+      const float2 a = make_float2(__fdiv_rn(x[4 * i], scale), __fdiv_rn(x[4 * i + 1], scale));
+      const float2 b = make_float2(__fdiv_rn(x[4 * i + 2], scale), __fdiv_rn(x[4 * i + 3], scale));
+      w[i] = (uint32_t)__nv_cvt_float2_to_fp8x2(a, __NV_SATFINITE, __NV_E4M3) |
+             ((uint32_t)__nv_cvt_float2_to_fp8x2(b, __NV_SATFINITE, __NV_E4M3) << 16);
     }
     if (on) {
       *reinterpret_cast<uint2*>(dst + 8 * j) = make_uint2(w[0], w[1]);
       *reinterpret_cast<uint2*>(dst + D / 2 + 8 * j) = make_uint2(w[2], w[3]);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint2 a = fp8x4_to_half4(w[2 * i]), b = fp8x4_to_half4(w[2 * i + 1]);
+      key[i] = make_uint4(a.x, a.y, b.x, b.y);
     }
   } else {
     // per 32-dim group (four lanes): scale = (max - min) / 15 and min in fp16, codes
@@ -217,12 +226,14 @@ __device__ __forceinline__ void store_kv_row(uint8_t* dst, float (&x)[16], float
       const __half hm = __float2half_rn(mn);
       const float s = __half2float(hs), m = __half2float(hm);
       uint32_t packed = 0;
+      float v[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float cf = fminf(fmaxf(rintf((x[8 * hf + i] - m) / s), 0.f), 15.f);
         packed |= (uint32_t)cf << (4 * i);
-        x[8 * hf + i] = fmaf(cf, s, m);
+        v[i] = fmaf(cf, s, m);
       }
+      key[hf] = pack8(v);
       if (on) {
         *reinterpret_cast<uint32_t*>(dst + hf * (D / 4) + 4 * j) = packed;
         if ((j & 3) == 0)
@@ -232,24 +243,77 @@ __device__ __forceinline__ void store_kv_row(uint8_t* dst, float (&x)[16], float
   }
 }
 
-// Eight stored values (dims 8 d8 ..) of a row of a page
+// Eight stored values (dims 8 d8 ..) of a row of a page, in the bounds' 16-bit type
 template <int D, int FMT>
-__device__ __forceinline__ void load_kv8(const uint8_t* row, int d8, float (&v)[8]) {
+__device__ __forceinline__ uint4 load_key8(const uint8_t* row, int d8) {
   if constexpr (FMT == kFmtBf16) {
-    unpack8(*reinterpret_cast<const uint4*>(row + 16 * d8), v);
+    return *reinterpret_cast<const uint4*>(row + 16 * d8);
   } else if constexpr (FMT == kFmtFp8) {
     const uint2 w = *reinterpret_cast<const uint2*>(row + 8 * d8);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[i] = fp8_to_f32((w.x >> (8 * i)) & 255u);
-      v[4 + i] = fp8_to_f32((w.y >> (8 * i)) & 255u);
-    }
+    const uint2 a = fp8x4_to_half4(w.x), b = fp8x4_to_half4(w.y);
+    return make_uint4(a.x, a.y, b.x, b.y);
   } else {
     const uint32_t w = *reinterpret_cast<const uint32_t*>(row + 4 * d8);
     const __half2 sm = *reinterpret_cast<const __half2*>(row + D / 2 + (d8 / 4) * 4);
     const float s = __low2float(sm), m = __high2float(sm);
+    float v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = fmaf((float)((w >> (4 * i)) & 15u), s, m);
+    return pack8(v);
+  }
+}
+
+// min / max of 16-bit pairs; a NaN stays
+template <int FMT, bool MAX>
+__device__ __forceinline__ uint32_t pick2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if constexpr (FMT == kFmtFp8) {
+    if constexpr (MAX) asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  } else {
+    if constexpr (MAX) asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  }
+  return r;
+}
+template <int FMT, bool MAX>
+__device__ __forceinline__ void pick8(uint4& a, const uint4& b) {
+  a.x = pick2<FMT, MAX>(a.x, b.x);
+  a.y = pick2<FMT, MAX>(a.y, b.y);
+  a.z = pick2<FMT, MAX>(a.z, b.z);
+  a.w = pick2<FMT, MAX>(a.w, b.w);
+}
+__device__ __forceinline__ uint4 shfl_xor4(const uint4& v, int o) {
+  return make_uint4(__shfl_xor_sync(0xffffffffu, v.x, o), __shfl_xor_sync(0xffffffffu, v.y, o),
+                    __shfl_xor_sync(0xffffffffu, v.z, o), __shfl_xor_sync(0xffffffffu, v.w, o));
+}
+// stores eight bounds: finite (infinities become the largest value, a NaN `nan`)
+template <int FMT>
+__device__ __forceinline__ void store_bound8(void* dst, const uint4& v, float nan) {
+  constexpr float kMax = FMT == kFmtFp8 ? 448.f : 3.3895313892515355e38f;
+  float x[8];
+  if constexpr (FMT == kFmtFp8) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      x[2 * i] = f.x;
+      x[2 * i + 1] = f.y;
+    }
+  } else {
+    unpack8(v, x);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = x[i] != x[i] ? nan * kMax : fminf(fmaxf(x[i], -kMax), kMax);
+  if constexpr (FMT == kFmtFp8) {
+    uint32_t w[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      w[i] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(x[4 * i], x[4 * i + 1]), __NV_SATFINITE, __NV_E4M3) |
+             ((uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(x[4 * i + 2], x[4 * i + 3]), __NV_SATFINITE, __NV_E4M3) << 16);
+    *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+  } else {
+    *reinterpret_cast<uint4*>(dst) = pack8(x);
   }
 }
 
@@ -258,32 +322,51 @@ __global__ void __launch_bounds__(128) append_kernel(AppendArgs a) {
   using S = AppendShape<D>;
   constexpr int kLanes = S::kLanes, kRows = S::kRows;
   constexpr int kRowB = PageRow<D, FMT>::kBytes;
+  constexpr int kHeads = 4;                // heads whose rows are in flight together
   __shared__ float s_rot[ROT == kRotPart ? kRows * D : 1];
-  __shared__ float s_k[S::kSpan * D];      // stored keys of the block's tokens
-  __shared__ int s_slot[S::kSpan];
-  __shared__ int s_run[S::kSpan + 1];      // token index of each run's first token
-  __shared__ int s_count[2];               // tokens, runs
+  __shared__ uint4 s_key[S::kSpan * (D / 8)];     // stored keys of the block's tokens
+  __shared__ int s_slot[S::kSpan + 1];            // [0]: the token before the tile
+  __shared__ int s_run[S::kSpan + 1];             // token of each run's start, then the end of the last
   pdl_launch();
   pdl_wait();
   const int tid = threadIdx.x;
   const int j = tid % kLanes, r0 = tid / kLanes;
-  const int tile0 = blockIdx.x * kRows;
+  // blocks of the q groups, then of the v groups, then of the k heads, tile by tile
+  const int tiles = (a.T + kRows - 1) / kRows, qv = tiles * (a.q_groups + a.v_groups);
+  const bool is_k = blockIdx.x >= qv;
+  const int tile = is_k ? a.k_tile : kRows;
+  const int k_tiles = (a.T + a.k_tile - 1) / a.k_tile;
+  const int block = is_k ? blockIdx.x - qv : blockIdx.x;
+  const int y = is_k ? block / k_tiles : block / tiles;
+  const int tile0 = (is_k ? block % k_tiles : block % tiles) * tile;
   const size_t page_b = (size_t)a.num_layers * 2 * a.KH * kPageTok * kRowB;
   float* scratch = s_rot + (ROT == kRotPart ? r0 * D : 0);
 
-  auto load_row = [&](int t, int head, float (&x)[16]) {
+  auto load_row = [&](int t, int head, uint4 (&x)[2]) {
     const __nv_bfloat16* src = reinterpret_cast<const __nv_bfloat16*>(a.qkv) + (size_t)t * a.ld_qkv + (size_t)head * D;
-    unpack8(*reinterpret_cast<const uint4*>(src + 8 * j), x);
-    unpack8(*reinterpret_cast<const uint4*>(src + D / 2 + 8 * j), x + 8);
+    x[0] = *reinterpret_cast<const uint4*>(src + 8 * j);
+    x[1] = *reinterpret_cast<const uint4*>(src + D / 2 + 8 * j);
   };
-  auto cos_row = [&](int t) -> const float* {
+  // row of the rotation table of token t; with a whole-head rotation this lane's 8 cos, 8 sin
+  auto cos_row = [&](int t, float (&cs)[16]) -> const float* {
     if (ROT == kRotNone) return nullptr;
     int p = a.positions[t];
     if (p < 0 || p >= a.max_pos) {           // outside the table: reported, nearest row taken
       report_error(a.err, kErrBounds);
       p = p < 0 ? 0 : a.max_pos - 1;
     }
-    return a.cos_sin + (size_t)p * a.rot_dim;
+    const float* row = a.cos_sin + (size_t)p * a.rot_dim;
+    if constexpr (ROT == kRotFull) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float4 v = *reinterpret_cast<const float4*>(row + (i / 2) * (D / 2) + 8 * j + 4 * (i % 2));
+        cs[4 * i] = v.x;
+        cs[4 * i + 1] = v.y;
+        cs[4 * i + 2] = v.z;
+        cs[4 * i + 3] = v.w;
+      }
+    }
+    return row;
   };
   auto page_of = [&](int slot) -> int {      // -1: not stored
     if (slot < 0) return -1;
@@ -299,156 +382,176 @@ __global__ void __launch_bounds__(128) append_kernel(AppendArgs a) {
            ((((size_t)a.layer * 2 + kv) * a.KH + head) * kPageTok + slot % kPageTok) * (size_t)kRowB;
   };
 
-  int y = blockIdx.y;
-  if (y < a.q_groups) {
-    // ---- q heads
+  if (!is_k && y >= a.q_groups) {
+    // ---- v heads
+    const int gv = y - a.q_groups;
     const int t = tile0 + r0;
-    const bool on = t < a.T;
-    const int h1 = min(a.Hq, (y + 1) * a.heads_per_group);
-    const float* cs = on ? cos_row(t) : a.cos_sin;
-    for (int h = y * a.heads_per_group; h < h1; ++h) {
-      float x[16];
-      load_row(on ? t : 0, h, x);
-      norm_rotate<D, ROT>(x, reinterpret_cast<const __nv_bfloat16*>(a.wq), a.eps, j, cs, a.rot_dim, scratch);
-      if (on) {
-        __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(a.q_out) + (size_t)t * a.ld_out + (size_t)h * D;
-        *reinterpret_cast<uint4*>(dst + 8 * j) = pack8(x);
-        *reinterpret_cast<uint4*>(dst + D / 2 + 8 * j) = pack8(x + 8);
+    const bool tok = t < a.T;
+    const int slot = tok ? a.slots[t] : -1;
+    const int h1 = min(a.KH, (gv + 1) * a.heads_per_group);
+    for (int h0 = gv * a.heads_per_group; h0 < h1; h0 += kHeads) {
+      uint4 in[kHeads][2];
+#pragma unroll
+      for (int i = 0; i < kHeads; ++i) load_row(tok ? t : tile0, a.Hq + a.KH + min(h0 + i, h1 - 1), in[i]);
+      const int page = page_of(slot);
+      const bool on = page >= 0;
+#pragma unroll
+      for (int i = 0; i < kHeads; ++i) {
+        if (h0 + i >= h1) break;
+        float x[16];
+        unpack8(in[i][0], x);
+        unpack8(in[i][1], x + 8);
+        const float sc = FMT == kFmtFp8 ? a.kv_scale[(a.layer * 2 + 1) * a.KH + h0 + i] : 1.f;
+        uint4 key[2];
+        store_kv_row<D, FMT>(on ? kv_row(page, slot, 1, h0 + i) : nullptr, x, sc, j, on, key);
       }
     }
     return;
   }
-  y -= a.q_groups;
-  if (y < a.v_groups) {
-    // ---- v heads
+  if (!is_k) {
+    // ---- q heads
     const int t = tile0 + r0;
-    const int slot = t < a.T ? a.slots[t] : -1;
-    const int page = page_of(slot);
-    const bool on = page >= 0;
-    const int h1 = min(a.KH, (y + 1) * a.heads_per_group);
-    for (int h = y * a.heads_per_group; h < h1; ++h) {
-      float x[16];
-      load_row(on ? t : 0, a.Hq + a.KH + h, x);
-      const float sc = FMT == kFmtFp8 ? a.kv_scale[(a.layer * 2 + 1) * a.KH + h] : 1.f;
-      store_kv_row<D, FMT>(on ? kv_row(page, slot, 1, h) : nullptr, x, sc, j, on);
+    const bool on = t < a.T;
+    const int ht = on ? t : tile0;           // rows without a token repeat the tile's first
+    float cs[16];
+    const float* row = cos_row(ht, cs);
+    const int h1 = min(a.Hq, (y + 1) * a.heads_per_group);
+    for (int h0 = y * a.heads_per_group; h0 < h1; h0 += kHeads) {
+      uint4 in[kHeads][2];
+#pragma unroll
+      for (int i = 0; i < kHeads; ++i) load_row(ht, min(h0 + i, h1 - 1), in[i]);
+#pragma unroll
+      for (int i = 0; i < kHeads; ++i) {
+        if (h0 + i >= h1) break;
+        float x[16];
+        unpack8(in[i][0], x);
+        unpack8(in[i][1], x + 8);
+        norm_rotate<D, ROT>(x, reinterpret_cast<const __nv_bfloat16*>(a.wq), a.eps, j, cs, row, a.rot_dim, scratch);
+        if (on) {
+          __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(a.q_out) + (size_t)t * a.ld_out + (size_t)(h0 + i) * D;
+          *reinterpret_cast<uint4*>(dst + 8 * j) = pack8(x);
+          *reinterpret_cast<uint4*>(dst + D / 2 + 8 * j) = pack8(x + 8);
+        }
+      }
     }
     return;
   }
   // ---- one k head
-  const int h = y - a.v_groups;
+  const int h = y;
   const float sc = FMT == kFmtFp8 ? a.kv_scale[(a.layer * 2 + 0) * a.KH + h] : 1.f;
-  int first = tile0, count = min(kRows, a.T - tile0);
+  const int in_tile = min(tile, a.T - tile0);
+  uint4 in[2];
+  load_row(r0 < in_tile ? tile0 + r0 : tile0, a.Hq + h, in);
+  int first = 0, last = in_tile, runs = 0;
   if (a.bounds != nullptr) {
-    // the tokens of the runs that begin in this tile
-    for (int i = tid; i < S::kSpan; i += 128) s_slot[i] = tile0 + i < a.T ? a.slots[tile0 + i] : -1;
-    __syncthreads();
-    if (tid == 0) {
-      auto joins = [&](int prev, int cur) { return prev >= 0 && cur == prev + 1 && cur % kPageTok != 0; };
-      int i = 0, runs = 0;
-      if (tile0 > 0) {
-        int prev = a.slots[tile0 - 1];
-        while (i < count && joins(prev, s_slot[i])) prev = s_slot[i++];
-      }
-      s_count[0] = i;                        // the first token of this block
-      int k = i;
-      for (; k < S::kSpan && tile0 + k < a.T; ++k) {
-        const bool j0 = k > i && joins(s_slot[k - 1], s_slot[k]);
-        if (k >= count && !j0) break;
-        if (!j0) s_run[runs++] = k;
-      }
-      s_run[runs] = k;
-      s_count[1] = runs;
+    if (tid <= in_tile + kPageTok - 1) {     // <= kSpan
+      const int i = tile0 + tid - 1;
+      s_slot[tid] = i >= 0 && i < a.T ? a.slots[i] : -1;
     }
     __syncthreads();
-    const int skip = s_count[0];
-    count = s_run[s_count[1]] - skip;
-    if (s_count[1] == 0) count = 0;
-    first = tile0 + skip;
+    // starts of runs, tokens in_tile .. in_tile + 14 included: a run has at most 16 tokens
+    const int lane = tid & 31;
+    uint64_t starts = 0;
+#pragma unroll
+    for (int k = 0; k < (S::kSpan + 31) / 32; ++k) {
+      const int i = 32 * k + lane;
+      bool st = true;
+      if (i < in_tile + kPageTok - 1 && tile0 + i < a.T) {
+        const int prev = s_slot[i], cur = s_slot[i + 1];
+        st = !(prev >= 0 && cur == prev + 1 && cur % kPageTok != 0);
+      }
+      starts |= (uint64_t)__ballot_sync(0xffffffffu, st) << (32 * k);
+    }
+    const uint64_t own = starts & ((1ull << in_tile) - 1);
+    runs = __popcll(own);
+    first = runs ? __ffsll((long long)own) - 1 : in_tile;
+    last = runs ? __ffsll((long long)(starts >> in_tile << in_tile)) - 1 : in_tile;
+    if (tid < in_tile && (own >> tid & 1)) s_run[__popcll(own & ((1ull << tid) - 1))] = tid;
+    if (tid == 0) s_run[runs] = last;
   }
-  for (int b = 0; b < count; b += kRows) {
-    const int t = first + b + r0;
-    const bool live = b + r0 < count;
+  for (int b = 0; b < last; b += kRows) {
+    const int k = b + r0, t = tile0 + k;     // this row's token
+    if (k >= in_tile && k < last) load_row(t, a.Hq + h, in);
+    const bool live = k >= first && k < last;
     const int slot = live ? a.slots[t] : -1;
+    float cs[16], x[16];
+    const float* row = cos_row(live ? t : tile0, cs);
+    unpack8(in[0], x);
+    unpack8(in[1], x + 8);
+    norm_rotate<D, ROT>(x, reinterpret_cast<const __nv_bfloat16*>(a.wk), a.eps, j, cs, row, a.rot_dim, scratch);
     const int page = page_of(slot);
     const bool on = page >= 0;
-    float x[16];
-    load_row(on ? t : 0, a.Hq + h, x);
-    norm_rotate<D, ROT>(x, reinterpret_cast<const __nv_bfloat16*>(a.wk), a.eps, j, on ? cos_row(t) : a.cos_sin,
-                        a.rot_dim, scratch);
-    store_kv_row<D, FMT>(on ? kv_row(page, slot, 0, h) : nullptr, x, sc, j, on);
+    uint4 key[2];
+    store_kv_row<D, FMT>(on ? kv_row(page, slot, 0, h) : nullptr, x, sc, j, on, key);
     if (a.bounds != nullptr && live) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s_k[(t - tile0) * D + (i < 8 ? 0 : D / 2 - 8) + 8 * j + i] = x[i];
+      s_key[k * (D / 8) + j] = key[0];
+      s_key[k * (D / 8) + D / 16 + j] = key[1];
     }
   }
   if (a.bounds == nullptr) return;
   __syncthreads();
-  // ---- bounds: D / 8 threads a run, 8 dims each; rows of the page before the run come
-  // from the pool (written by earlier calls), the run's own from shared memory
-  constexpr int kTpr = D / 8;
-  constexpr float kMax = FMT == kFmtFp8 ? 448.f : 3.3895313892515355e38f;
-  const int d8 = tid % kTpr;
-  for (int run = tid / kTpr; run < s_count[1]; run += 128 / kTpr) {
+  // ---- bounds: one warp a run, D / 8 lanes a row.  The rows of the page before the run
+  // come from the pool (written by earlier calls), the run's own from shared memory.
+  constexpr int kPer = D / 8, kGroups = 32 / kPer;
+  const int lane = tid & 31, d8 = lane % kPer, grp = lane / kPer;
+  for (int run = tid / 32; run < runs; run += 4) {
     const int k0 = s_run[run], k1 = s_run[run + 1];
-    const int slot = s_slot[k0];
+    const int slot = s_slot[k0 + 1];
     const int page = slot >= 0 && slot / kPageTok < a.num_pages ? slot / kPageTok : -1;
     if (page < 0) continue;
-    float lo[8], hi[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      lo[i] = INFINITY;
-      hi[i] = -INFINITY;
-    }
-    auto take = [&](const float (&v)[8]) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const bool nan = v[i] != v[i];         // a NaN key may score anything
-        lo[i] = fminf(lo[i], nan ? -kMax : v[i]);
-        hi[i] = fmaxf(hi[i], nan ? kMax : v[i]);
-      }
-    };
+    constexpr uint32_t kInf = FMT == kFmtFp8 ? 0x7C007C00u : 0x7F807F80u;
+    uint4 lo = make_uint4(kInf, kInf, kInf, kInf), hi = lo;
+    hi.x = hi.y = hi.z = hi.w = kInf | 0x80008000u;
     const uint8_t* base = kv_row(page, 0, 0, h);
     const int old = slot % kPageTok;
-#pragma unroll 5
-    for (int r = 0; r < old; ++r) {
-      float v[8];
-      load_kv8<D, FMT>(base + r * kRowB, d8, v);
-      take(v);
-    }
-    for (int k = k0; k < k1; ++k) {
-      float v[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = s_k[k * D + 8 * d8 + i];
-      take(v);
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      lo[i] = fminf(fmaxf(lo[i], -kMax), kMax);
-      hi[i] = fminf(fmaxf(hi[i], -kMax), kMax);
-    }
-    const size_t at = (((size_t)page * a.num_layers + a.layer) * a.KH + h) * 2 * D + 8 * d8;
-    if constexpr (FMT == kFmtFp8) {
-      uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        w[i / 4] |= (uint32_t)__nv_cvt_float_to_fp8(lo[i], __NV_SATFINITE, __NV_E4M3) << (8 * (i % 4));
-        w[2 + i / 4] |= (uint32_t)__nv_cvt_float_to_fp8(hi[i], __NV_SATFINITE, __NV_E4M3) << (8 * (i % 4));
+    for (int r = 0; r < kPageTok; r += kGroups) {
+      if (r + grp < old) {
+        const uint4 v = load_key8<D, FMT>(base + (r + grp) * kRowB, d8);
+        pick8<FMT, false>(lo, v);
+        pick8<FMT, true>(hi, v);
       }
-      uint8_t* dst = reinterpret_cast<uint8_t*>(a.bounds) + at;
-      *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
-      *reinterpret_cast<uint2*>(dst + D) = make_uint2(w[2], w[3]);
-    } else {
-      __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(a.bounds) + at;
-      *reinterpret_cast<uint4*>(dst) = pack8(lo);
-      *reinterpret_cast<uint4*>(dst + D) = pack8(hi);
+    }
+    for (int k = k0 + grp; k < k1; k += kGroups) {
+      const uint4 v = s_key[k * (D / 8) + d8];
+      pick8<FMT, false>(lo, v);
+      pick8<FMT, true>(hi, v);
+    }
+#pragma unroll
+    for (int o = kPer; o < 32; o <<= 1) {
+      pick8<FMT, false>(lo, shfl_xor4(lo, o));
+      pick8<FMT, true>(hi, shfl_xor4(hi, o));
+    }
+    if (grp == 0) {
+      constexpr int kEl = FMT == kFmtFp8 ? 1 : 2;
+      uint8_t* dst = reinterpret_cast<uint8_t*>(a.bounds) +
+                     ((((size_t)page * a.num_layers + a.layer) * a.KH + h) * 2 * D + 8 * d8) * kEl;
+      store_bound8<FMT>(dst, lo, -1.f);
+      store_bound8<FMT>(dst + D * kEl, hi, 1.f);
     }
   }
 }
 
 template <int D, int FMT>
-static void launch_append(const AppendArgs& a, cudaStream_t st) {
+static void launch_append(AppendArgs a, cudaStream_t st) {
+  // heads of a q or v block: the rotation table's row is read once a block, so as many as
+  // leave a block to every SM (B200, 32 + 8 heads, us with 4 / 8 / 16 heads a block: 512 tokens
+  // 5.0 / 6.7 / 9.2, 2048 tokens 14.6 / 13.1 / 12.9; 8192 tokens with all 32: 30.0, with 4: 32.5)
   const int tiles = (a.T + AppendShape<D>::kRows - 1) / AppendShape<D>::kRows;
-  const dim3 grid(tiles, a.q_groups + a.v_groups + a.KH);
+  int per = 4;
+  while (per < a.Hq && (long long)tiles * ((a.Hq + 2 * per - 1) / (2 * per)) >= device_sm_count()) per *= 2;
+  a.heads_per_group = per;
+  a.q_groups = (a.Hq + per - 1) / per;
+  a.v_groups = (a.KH + per - 1) / per;
+  // In a decode step each token is a run whose page is read back, one warp a run: small k
+  // tiles spread them.  In a prompt a run has 16 tokens, and most small tiles have none.
+  // B200, us with tiles of 4 / 8 / 16: decode of 64 rows (fp8) 4.5 / 6.0 / 8.2, of 512 rows
+  // 10.2 / 8.0 / 11.3; prompts of 512 tokens 5.9 / 4.1 / 5.1, of 2048 22.6 / 17.3 / 16.1.
+  a.k_tile = a.bounds == nullptr || a.T > 768 ? 16 : a.T > 256 ? 8 : 4;
+  const long long k_blocks = (long long)((a.T + a.k_tile - 1) / a.k_tile) * a.KH;
+  const long long blocks = k_blocks + (long long)tiles * (a.q_groups + a.v_groups);
+  VRM_REQUIRE(blocks <= INT_MAX, "qk_norm_rope_kv_write: too many tokens");
+  const dim3 grid((unsigned)blocks);
   if (a.rot_dim == 0) launch_kernel(append_kernel<D, FMT, kRotNone>, grid, dim3(128), 0, st, a);
   else if (a.rot_dim == D) launch_kernel(append_kernel<D, FMT, kRotFull>, grid, dim3(128), 0, st, a);
   else launch_kernel(append_kernel<D, FMT, kRotPart>, grid, dim3(128), 0, st, a);
@@ -459,10 +562,6 @@ void qk_norm_rope_kv_write(const AppendArgs& in, cudaStream_t st) {
   AppendArgs a = in;
   a.err = error_word();
   VRM_REQUIRE(a.D == 64 || a.D == 128, "qk_norm_rope_kv_write: head_dim must be 64 or 128");
-  a.heads_per_group = 4;
-  a.q_groups = (a.Hq + a.heads_per_group - 1) / a.heads_per_group;
-  a.v_groups = (a.KH + a.heads_per_group - 1) / a.heads_per_group;
-  VRM_REQUIRE(a.q_groups + a.v_groups + a.KH <= 65535, "qk_norm_rope_kv_write: too many heads");
   auto go = [&](auto d) {
     constexpr int D = decltype(d)::value;
     if (a.fmt == kFmtQ4) launch_append<D, kFmtQ4>(a, st);
@@ -477,19 +576,26 @@ void qk_norm_rope_kv_write(const AppendArgs& in, cudaStream_t st) {
 // ================================================================ page selection
 // Score of page p for the group's heads g:  sum_d (up_d * max_pd + dn_d * min_pd) with
 // up_d = sum_g max(q_gd, 0), dn_d = sum_g min(q_gd, 0): no key of the page gives the group
-// a larger sum of scores.  Which page is the last to be taken depends on differences of
-// any size, so scores are summed in 64 bits, where products of 8-bit significands are
-// exact, and the choice is the one exact arithmetic makes, ties to the lowest page.
+// a larger sum of scores.
 //
-// A bound becomes a double by moving its sign, exponent and significand bits into place
-// without re-biasing the exponent: the same value times 2^-896 (bf16) or 2^-1016 (e4m3),
-// zeros and subnormals included.  The common factor (up and dn carry 2^800 against
-// underflow) does not change an order.
+// Which page is the last to be taken depends on differences of any size, so the choice is
+// the one that 64-bit sums make (products of 8-bit significands are exact there), ties to
+// the lowest page.  64-bit arithmetic for every page would cost more than reading it, so
+// pages are first scored in fp32 by the tensor cores: 16 pages are the rows of an MMA, their
+// bounds go from memory to its A operand as they are, and the query vector is split into
+// three 16-bit parts (24 bits of it) that fill three of the eight columns.  With S an upper
+// bound of sum |term|, such a score is off by less than E = 2^-18 S (an MMA from zero adds 16
+// exact products, each off by at most 2^-23 of their largest magnitude: 2^-19 S over all of
+// them, and the 18 fp32 additions of their sums 2^-19.8 S), so with the need-th largest score b every page above b + 2E is taken,
+// every page below b - 2E is not, and the few between are scored again in 64 bits.
+// Whatever fp32 cannot decide (S out of range, non-finite values, more pages between
+// than kSelList) is decided by 64-bit scores of all pages.
 namespace {
 
-constexpr int kSelThreads = 256;
-
-
+// A bound becomes a double by moving its sign, exponent and significand bits into place
+// without re-biasing the exponent: the same value times 2^-896 (bf16) or 2^-1016 (e4m3),
+// zeros and subnormals included; the query side carries 2^800 against underflow.  The
+// common factor does not change an order.
 __device__ __forceinline__ double hi_word(uint32_t h) { return __hiloint2double((int)h, 0); }
 
 // the two bf16 of w
@@ -503,206 +609,573 @@ __device__ __forceinline__ void fp8x4_to_f64(uint32_t w, double (&v)[4]) {
   for (int i = 0; i < 4; ++i) v[i] = hi_word((uint32_t)((int32_t)(w << (24 - 8 * i)) >> 7) & 0x80FE0000u);
 }
 
+__device__ __forceinline__ uint32_t max_abs_half2(uint32_t a, uint32_t b) {
+  const __half2 r = __hmax2(__habs2(*reinterpret_cast<__half2*>(&a)), __habs2(*reinterpret_cast<__half2*>(&b)));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// unsigned keys in the order of the values
 __device__ __forceinline__ uint64_t sortable(double s) {
   if (s != s) return ~0ull;                      // a NaN is read first: it is not hidden
   const uint64_t b = (uint64_t)__double_as_longlong(s + 0.0);   // -0 counts as 0
   return (b >> 63) ? ~b : b | (1ull << 63);
 }
+__device__ __forceinline__ uint32_t sortable(float s) {
+  const uint32_t b = __float_as_uint(s + 0.f);
+  return (b >> 31) ? ~b : b | (1u << 31);
+}
+__device__ __forceinline__ float from_sortable(uint32_t k) { return __uint_as_float(k >> 31 ? k & 0x7fffffffu : ~k); }
+
+constexpr int kSelList = 128;                    // pages decided by the short 64-bit path
+constexpr int kSelMaxPages = 24576;              // candidate pages of a row (8 bytes of shared memory each)
+constexpr int kBins = 1024;
+
+template <int NT>
+struct SelectScratch {
+  __align__(16) uint32_t hist[kBins];
+  uint32_t scan[NT / 32];
+  uint64_t red[2][NT / 32];
+  uint32_t border, left, in_bin;
+};
+
+// Where the need-th largest of a set of keys lies: it shares the bits `mask` of `prefix`,
+// and is the left-th largest of the `in_bin` keys that do.
+template <typename K>
+struct Border {
+  K prefix, mask;
+  int shift;                                     // lowest bit of mask
+  uint32_t left, in_bin;
+  // from the largest and the smallest key: the bits they share are settled
+  __device__ __forceinline__ void start(K top, K low, uint32_t need, int n) {
+    const K differ = top ^ low;
+    shift = differ ? 64 - __clzll((unsigned long long)differ) : 0;
+    mask = shift >= (int)sizeof(K) * 8 ? (K)0 : (K)(~(K)0 << shift);
+    prefix = top & mask;
+    left = need;
+    in_bin = (uint32_t)n;
+  }
+};
+
+// One histogram of the bins bin(0) .. bin(n - 1) (-1: not counted): sc.border becomes the bin
+// of the left-th entry from the top, which is its sc.left-th of sc.in_bin.  The bins are
+// zero before and after.
+template <int NT, typename F>
+__device__ __forceinline__ void radix_count(SelectScratch<NT>& sc, int n, uint32_t left, F bin) {
+  constexpr int kPer = kBins / NT;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  for (int i0 = tid; i0 < n; i0 += 8 * NT) {
+    int b[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) b[q] = i0 + q * NT < n ? bin(i0 + q * NT) : -1;
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      if (b[q] >= 0) atomicAdd(&sc.hist[b[q] % kPer * NT + b[q] / kPer], 1u);
+  }
+  __syncthreads();
+  // suffix sums: thread tid adds up the kPer bins below kBins - tid * kPer
+  uint32_t c[kPer], sum = 0;
+#pragma unroll
+  for (int q = 0; q < kPer; ++q) {
+    uint32_t* p = &sc.hist[q * NT + NT - 1 - tid];
+    c[q] = *p;
+    *p = 0u;
+    sum += c[q];
+  }
+  uint32_t incl = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t v = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) sc.scan[warp] = incl;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < NT / 32; ++w) incl += w < warp ? sc.scan[w] : 0u;
+  uint32_t before = incl - sum;
+  if (before < left && incl >= left) {           // one thread
+#pragma unroll
+    for (int q = kPer - 1; q >= 0; --q) {
+      if (before < left && before + c[q] >= left) {
+        sc.border = kBins - (tid + 1) * kPer + q;
+        sc.left = left - before;
+        sc.in_bin = c[q];
+      }
+      before += c[q];
+    }
+  }
+  __syncthreads();
+}
+
+// Settles up to 10 more bits of the border of keys key(0) .. key(n - 1)
+template <int NT, typename K, typename F>
+__device__ __forceinline__ void radix_pass(SelectScratch<NT>& sc, int n, F key, Border<K>& b) {
+  const int low = max(0, b.shift - 10);
+  radix_count<NT>(sc, n, b.left, [&](int i) -> int {
+    const K k = key(i);
+    return (k & b.mask) == b.prefix ? (int)((k & (K)~b.mask) >> low) : -1;
+  });
+  b.prefix |= (K)sc.border << low;
+  b.left = sc.left;
+  b.in_bin = sc.in_bin;
+  b.shift = low;
+  b.mask = (K)(~(K)0 << low);
+  __syncthreads();
+}
 
 }  // namespace
 
-template <int D, bool F8>
-__global__ void __launch_bounds__(kSelThreads) select_kernel(SelectArgs a) {
+// One cluster of 1, 2, 4 or 8 CTAs per (kv head, query row).  Every CTA scores a slice of
+// the row's candidate pages, 16 a warp at a time: lane (g, c) reads 16-byte pieces c, c + 4,
+// ... of pages g and g + 8, and each piece of the next 16 pages is requested as soon as the
+// MMAs have used the present one.  Scores go to the shared memory of the cluster's first
+// CTA, which chooses.
+template <int D, bool F8, int NT>
+__global__ void __launch_bounds__(NT, 512 / NT) select_kernel(SelectArgs a) {
   constexpr int kEl = F8 ? 1 : 2;
-  constexpr int kLaneB = D * kEl / 8;            // bytes of a min (or max) row per lane, 8 lanes a page
-  constexpr int kDims = D / 8;                   // dims per lane
-  extern __shared__ __align__(16) uint64_t s_key[];    // [candidates]
-  __shared__ double s_up[D], s_dn[D];
-  __shared__ uint32_t s_hist[256];
-  __shared__ uint64_t s_sel[2];                  // prefix; entries still to take
-  __shared__ uint32_t s_scan[kSelThreads / 32];
+  constexpr int kPageB = 2 * D * kEl;            // bounds of one page and kv head
+  constexpr int kPieces = kPageB / 64;           // 16-byte pieces of a page per lane
+  constexpr int kSteps = 2 * D / 16;             // MMAs of 16 pages
+  constexpr int kSp = kSteps / kPieces;          // MMAs a piece feeds
+  constexpr int kWarps = NT / 32;
+  extern __shared__ __align__(16) uint8_t s_dyn[];
+  float* s_score = reinterpret_cast<float*>(s_dyn);              // [max_pages] fp32 scores
+  int* s_page = reinterpret_cast<int*>(s_dyn) + a.max_pages;     // [max_pages] their pages in the pool
+  uint64_t* s_key = reinterpret_cast<uint64_t*>(s_dyn);          // or 64-bit keys, over both
+  __shared__ SelectScratch<NT> sc;
+  __shared__ double s_q[2 * D];                  // dn, up
+  __shared__ __align__(8) uint16_t s_part[3][2 * D];             // their three 16-bit parts
+  __shared__ float s_norm[2][kWarps];
+  __shared__ uint32_t s_ends[8 * kWarps][3];     // per CTA and warp: largest key, ~smallest key, largest |bound|
+  __shared__ uint32_t s_cnt[2][kWarps];
+  __shared__ uint64_t s_lkey[kSelList];
+  __shared__ int s_lidx[kSelList], s_near[kSelList];
+  __shared__ float s_lval[kSelList], s_b;
+  __shared__ uint32_t s_count, s_nears;
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
   pdl_launch();
   pdl_wait();
-  const int kvh = blockIdx.x, t = blockIdx.y;
+  const int kvh = blockIdx.y, t = blockIdx.z;
+  const int nc = gridDim.x, rank = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int g = lane >> 2, c = lane & 3;
+
+  // the query vector's loads go out beside the load of the row's length
+  __nv_bfloat16 qv[8];
+#pragma unroll
+  for (int h = 0; h < 8; ++h)
+    qv[h] = tid < D && h < a.G ? reinterpret_cast<const __nv_bfloat16*>(a.q)[(size_t)t * a.ld_q + (size_t)(kvh * a.G + h) * D + tid]
+                               : __nv_bfloat16(0.f);
+  for (int i = tid; i < kBins / 4; i += NT) reinterpret_cast<uint4*>(sc.hist)[i] = make_uint4(0u, 0u, 0u, 0u);
+  // and, where the warp's first pages do not depend on it, beside its block-table entries
+  const bool early = nc == 1 && a.cu_q == nullptr;
+  const int first = a.sinks + warp * 16 + lane;
+  const int early_entry = early && lane < 16 && first < a.max_pages ? a.block_tables[(size_t)t * a.bt_stride + first] : 0;
   RowOf row;
-  if (!find_row(t, a.cu_q, a.context_lens, a.B, row)) return;
+  if (!find_row(t, a.cu_q, a.context_lens, a.B, row)) return;      // the same for the whole cluster
   int* out = a.out + ((size_t)t * a.KH + kvh) * a.budget;
   int total = row.n <= 0 ? 0 : (int)(((long long)row.n + kPageTok - 1) / kPageTok);
   total = min(total, a.max_pages);
   if (total <= a.budget) {
-    for (int i = tid; i < a.budget; i += kSelThreads) out[i] = i < total ? i : -1;
+    for (int i = rank * NT + tid; i < a.budget; i += nc * NT) out[i] = i < total ? i : -1;
     return;
   }
   const int need = a.budget - a.sinks - a.recent;
-  const int m = total - a.sinks - a.recent;      // candidates: pages sinks .. sinks + m - 1, m > need
-  for (int i = tid; i < a.sinks; i += kSelThreads) out[i] = i;
-  for (int i = tid; i < a.recent; i += kSelThreads) out[a.budget - a.recent + i] = total - a.recent + i;
+  const int n = total - a.sinks - a.recent;      // candidates: pages sinks .. sinks + n - 1, n > need
+  if (rank == 0) {
+    for (int i = tid; i < a.sinks; i += NT) out[i] = i;
+    for (int i = tid; i < a.recent; i += NT) out[a.budget - a.recent + i] = total - a.recent + i;
+  }
   if (need <= 0) return;
+  if (nc > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // this CTA runs
 
-  for (int d = tid; d < D; d += kSelThreads) {
-    const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(a.q) + (size_t)t * a.ld_q + (size_t)kvh * a.G * D + d;
-    double up = 0., dn = 0.;
-    for (int g = 0; g < a.G; ++g) {
-      const double x = (double)__bfloat162float(q[(size_t)g * D]);
-      if (x >= 0.) up += x;
-      else dn += x;                              // NaN lands here and spoils every score
+  const int slice = (n + nc - 1) / nc;
+  const int c0 = min(n, rank * slice), m = min(n, c0 + slice) - c0;
+  const int* bt = a.block_tables + (size_t)row.seq * a.bt_stride + a.sinks;
+  const size_t page_stride = (size_t)a.num_layers * a.KH * kPageB;
+  const uint8_t* bounds = reinterpret_cast<const uint8_t*>(a.bounds) + ((size_t)a.layer * a.KH + kvh) * kPageB;
+  bool odd = false;                              // something that fp32 scores cannot decide
+
+  // lanes 0..15 hold the block-table entries of the warp's 16 pages
+  auto entries = [&](int tile) -> int {
+    const int i = tile * 16 + lane;
+    return lane < 16 && i < m ? bt[c0 + i] : 0;
+  };
+  const uint8_t *p0, *p1;                        // this lane's pieces of pages g, g + 8
+  int* page0 = nullptr;
+  auto point = [&](int entry, int tile) {
+    const bool bad = entry < 0 || entry >= a.num_pages;
+    if (bad) report_error(a.err, kErrBounds);
+    odd |= bad;
+    entry = bad ? 0 : entry;
+    if (lane < 16 && tile * 16 + lane < m) page0[c0 + tile * 16 + lane] = entry;
+    p0 = bounds + (size_t)__shfl_sync(0xffffffffu, entry, g) * page_stride + c * 16;
+    p1 = bounds + (size_t)__shfl_sync(0xffffffffu, entry, g + 8) * page_stride + c * 16;
+  };
+  const int tiles = (m + 15) / 16;
+  uint32_t r[kPieces][2][4];
+  int entry0 = warp < tiles ? (early ? (warp * 16 + lane < m ? early_entry : 0) : entries(warp)) : 0;
+  if (nc > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");   // the first CTA runs
+  float* score0 = nc > 1 ? cluster.map_shared_rank(s_score, 0) : s_score;
+  page0 = nc > 1 ? cluster.map_shared_rank(s_page, 0) : s_page;
+  int next = 0;
+  if (warp < tiles) {
+    point(entry0, warp);
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      ld_stream<16>(r[i][0], p0 + i * 64);
+      ld_stream<16>(r[i][1], p1 + i * 64);
     }
-    const double f = __hiloint2double((1023 + 800) << 20, 0);
-    s_up[d] = up * f;
-    s_dn[d] = dn * f;
+    next = entries(warp + kWarps);
+  }
+  double qu = 0., qd = 0.;
+#pragma unroll
+  for (int h = 0; h < 8; ++h) {
+    const double x = (double)__bfloat162float(qv[h]);
+    if (x >= 0.) qu += x;
+    else qd += x;                                // NaN lands here and spoils every score
+  }
+
+  // up and dn times the power of two that brings the largest to [1, 2), in three parts
+  {
+    float mx = (float)fmax(qu, -qd), sum = (float)(qu - qd);
+    if (qd != qd) mx = sum = NAN;
+    odd |= mx != mx;
+    mx = warp_max(mx);
+    sum = warp_sum(sum);
+    if (lane == 0) {
+      s_norm[0][warp] = mx;
+      s_norm[1][warp] = sum;
+    }
   }
   __syncthreads();
-
-  const int sub = lane & 7, grp = lane >> 3;     // 8 lanes a page, 4 pages a warp
-  double up[kDims], dn[kDims];
+  float qmax = 0.f, l1 = 0.f;
 #pragma unroll
-  for (int i = 0; i < kDims; ++i) {
-    // 16-byte chunk i / (16 / kEl) of the lane: chunks are dealt round-robin to the lanes
-    constexpr int kPer = kLaneB >= 16 ? 16 / kEl : kDims;
-    const int d = (i / kPer) * (8 * kPer) + sub * kPer + i % kPer;
-    up[i] = s_up[d];
-    dn[i] = s_dn[d];
+  for (int w = 0; w < kWarps; ++w) {
+    qmax = fmaxf(qmax, s_norm[0][w]);
+    l1 += s_norm[1][w];
   }
-  const int* bt = a.block_tables + (size_t)row.seq * a.bt_stride + a.sinks;
-  for (int i0 = warp * 4; i0 < m; i0 += kSelThreads / 32 * 4) {
-    const int i = i0 + grp;
-    int page = i < m ? bt[i] : -1;
-    const bool bad = i < m && (page < 0 || page >= a.num_pages);
-    if (bad) report_error(a.err, kErrBounds);
-    if (bad) page = -1;
-    double s = 0.;
-    if (page >= 0) {
-      const uint8_t* b = reinterpret_cast<const uint8_t*>(a.bounds) +
-                         (((size_t)page * a.num_layers + a.layer) * a.KH + kvh) * (size_t)(2 * D * kEl);
-      constexpr int kChunks = kLaneB >= 16 ? kLaneB / 16 : 1;
+  const int e = (int)(__float_as_uint(qmax) >> 23);
+  // f16 parts: another 2^14, so that the last one stays above the subnormals
+  const double f = __hiloint2double((1023 + 127 + (F8 ? 14 : 0) - min(max(e, 1), 254)) << 20, 0);
+  l1 *= (float)f;
+  if (tid < D) {
+    s_q[tid] = qd * __hiloint2double((1023 + 800) << 20, 0);
+    s_q[D + tid] = qu * __hiloint2double((1023 + 800) << 20, 0);
 #pragma unroll
-      for (int c = 0; c < kChunks; ++c) {
-        if constexpr (!F8) {
-          const uint4 lo = ld_stream16(b + c * 128 + sub * 16), hi = ld_stream16(b + D * kEl + c * 128 + sub * 16);
-          const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
+    for (int k = 0; k < 2; ++k) {
+      float x = (float)((k ? qu : qd) * f);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            double x0, x1, y0, y1;
-            bf16x2_to_f64(wl[k], x0, x1);
-            bf16x2_to_f64(wh[k], y0, y1);
-            s = fma(dn[c * 8 + 2 * k], x0, s);
-            s = fma(dn[c * 8 + 2 * k + 1], x1, s);
-            s = fma(up[c * 8 + 2 * k], y0, s);
-            s = fma(up[c * 8 + 2 * k + 1], y1, s);
-          }
+      for (int part = 0; part < 3; ++part) {
+        if constexpr (F8) {
+          const __half h = __float2half_rn(x);
+          s_part[part][k * D + tid] = __half_as_ushort(h);
+          x -= __half2float(h);
         } else {
-          uint32_t wl[4], wh[4];
-          if constexpr (kLaneB == 16) {
-            const uint4 lo = ld_stream16(b + sub * 16), hi = ld_stream16(b + D + sub * 16);
-            wl[0] = lo.x, wl[1] = lo.y, wl[2] = lo.z, wl[3] = lo.w;
-            wh[0] = hi.x, wh[1] = hi.y, wh[2] = hi.z, wh[3] = hi.w;
-          } else {
-            const uint2 lo = ld_stream8(b + sub * 8), hi = ld_stream8(b + D + sub * 8);
-            wl[0] = lo.x, wl[1] = lo.y;
-            wh[0] = hi.x, wh[1] = hi.y;
-          }
-#pragma unroll
-          for (int k = 0; k < kDims / 4; ++k) {
-            double x[4], z[4];
-            fp8x4_to_f64(wl[k], x);
-            fp8x4_to_f64(wh[k], z);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              s = fma(dn[4 * k + e], x[e], s);
-              s = fma(up[4 * k + e], z[e], s);
-            }
-          }
+          const __nv_bfloat16 h = __float2bfloat16_rn(x);
+          s_part[part][k * D + tid] = __bfloat16_as_ushort(h);
+          x -= __bfloat162float(h);
         }
       }
     }
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (sub == 0 && i < m) s_key[i] = bad ? 0ull : sortable(s);
   }
   __syncthreads();
+  // B operand: column g < 3 is part g; step s takes four elements of the bounds' order
+  uint2 qb[kSteps];
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s) {
+    const int el = ((s / kSp) * 4 + c) * (16 / kEl) + (s % kSp) * 4;
+    qb[s] = g < 3 ? *reinterpret_cast<const uint2*>(&s_part[g < 3 ? g : 0][el]) : make_uint2(0u, 0u);
+  }
 
-  // radix selection of the need-th largest key, 8 bits a pass from the top
-  uint64_t prefix = 0, left = (uint64_t)need;
-  int shift = 56;
-  bool all = false;                              // every key with this prefix is taken
-  for (;; shift -= 8) {
-    s_hist[tid] = 0;
-    __syncthreads();
-    const uint64_t mask = shift == 56 ? 0ull : ~0ull << (shift + 8);
-    for (int i = tid; i < m; i += kSelThreads) {
-      const uint64_t k = s_key[i];
-      if ((k & mask) == prefix) atomicAdd(&s_hist[(k >> shift) & 255], 1u);
+  uint32_t key_hi = 0, key_lo_c = 0;             // largest key, largest complement
+  uint32_t amax = 0;                             // largest |bound| of the lane, both halves
+  for (int tile = warp; tile < tiles; tile += kWarps) {
+    const bool more = tile + kWarps < tiles;
+    if (more) {
+      point(next, tile + kWarps);
+      next = entries(tile + 2 * kWarps);
     }
-    __syncthreads();
-    // suffix sums over the 256 bins: thread tid owns bin 255 - tid
-    const uint32_t c = s_hist[255 - tid];
-    uint32_t incl = c;
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t v = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += v;
-    }
-    if (lane == 31) s_scan[warp] = incl;
-    __syncthreads();
-    for (int w = 0; w < warp; ++w) incl += s_scan[w];
-    if (incl >= left && incl - c < left) {
-      s_sel[0] = prefix | ((uint64_t)(255 - tid) << shift);
-      s_sel[1] = (left - (incl - c)) | (incl == left ? 1ull << 63 : 0ull);
-    }
-    __syncthreads();
-    prefix = s_sel[0];
-    left = s_sel[1] & ~(1ull << 63);
-    all = s_sel[1] >> 63;
-    if (all || shift == 0) break;
-  }
-  // keys above the prefix are taken, and of those that share it the first `left`
-  const uint64_t mask = ~0ull << shift;
-  const int per = (m + kSelThreads - 1) / kSelThreads;
-  const int i0 = min(m, tid * per), i1 = min(m, i0 + per);
-  uint32_t gt = 0, eq = 0;
-  for (int i = i0; i < i1; ++i) {
-    const uint64_t k = s_key[i] & mask;
-    gt += k > prefix;
-    eq += k == prefix;
-  }
-  // exclusive prefix of (gt, eq) over the threads, 16 bits each would overflow: two scans
-  __shared__ uint32_t s_scan2[kSelThreads / 32];
-  uint32_t ig = gt, ie = eq;
+    for (int i = 0; i < kPieces; ++i) {
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const uint32_t vg = __shfl_up_sync(0xffffffffu, ig, o), ve = __shfl_up_sync(0xffffffffu, ie, o);
-    if (lane >= o) {
-      ig += vg;
-      ie += ve;
+      for (int w = 0; w < kSp; ++w) {
+        const int s = i * kSp + w;
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+        if constexpr (F8) {
+          const uint32_t a0 = fp8x2_to_half2(r[i][0][w]), a1 = fp8x2_to_half2(r[i][1][w]);
+          const uint32_t a2 = fp8x2_to_half2(r[i][0][w] >> 16), a3 = fp8x2_to_half2(r[i][1][w] >> 16);
+          mma_f16(acc, a0, a1, a2, a3, qb[s].x, qb[s].y);
+          amax = max_abs_half2(max_abs_half2(amax, a0), max_abs_half2(a1, max_abs_half2(a2, a3)));
+        } else {
+          mma_bf16_16816(acc, r[i][0][2 * w], r[i][1][2 * w], r[i][0][2 * w + 1], r[i][1][2 * w + 1], qb[s].x, qb[s].y);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sum[k] += acc[k];
+      }
+      if constexpr (!F8) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          amax = __vmaxu2(amax, __vmaxu2(r[i][0][w] & 0x7fff7fffu, r[i][1][w] & 0x7fff7fffu));
+      }
+      if (more) {
+        ld_stream<16>(r[i][0], p0 + i * 64);
+        ld_stream<16>(r[i][1], p1 + i * 64);
+      }
+    }
+    // columns 0, 1 lie in lanes c = 0, column 2 in c = 1
+    float v0 = sum[0] + sum[1], v1 = sum[2] + sum[3];
+    v0 += __shfl_xor_sync(0xffffffffu, v0, 1);
+    v1 += __shfl_xor_sync(0xffffffffu, v1, 1);
+    const int i0 = tile * 16 + g;
+    if (c == 0) {
+      odd |= (i0 < m && !isfinite(v0)) || (i0 + 8 < m && !isfinite(v1));
+      if (i0 < m) {
+        score0[c0 + i0] = v0;
+        key_hi = max(key_hi, sortable(v0));
+        key_lo_c = max(key_lo_c, ~sortable(v0));
+      }
+      if (i0 + 8 < m) {
+        score0[c0 + i0 + 8] = v1;
+        key_hi = max(key_hi, sortable(v1));
+        key_lo_c = max(key_lo_c, ~sortable(v1));
+      }
     }
   }
-  if (lane == 31) {
-    s_scan[warp] = ig;
-    s_scan2[warp] = ie;
+  // infinite or NaN bounds (as bit patterns they are the largest), or fp32 cannot decide
+  uint32_t big = max(amax << 16, amax & 0xFFFF0000u);
+  if constexpr (F8) {
+    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&amax));
+    big = __float_as_uint(fmaxf(fabsf(v.x), fabsf(v.y)));
+  }
+  if (__any_sync(0xffffffffu, odd)) big = 0x7F800000u;
+  big = __reduce_max_sync(0xffffffffu, big);
+  key_hi = __reduce_max_sync(0xffffffffu, key_hi);
+  key_lo_c = __reduce_max_sync(0xffffffffu, key_lo_c);
+  if (lane < 3)
+    (nc > 1 ? cluster.map_shared_rank(&s_ends[0][0], 0) : &s_ends[0][0])[(rank * kWarps + warp) * 3 + lane] =
+        lane == 0 ? key_hi : lane == 1 ? key_lo_c : big;
+  if (tid == 0) s_count = s_nears = 0;
+  if (nc > 1) {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    if (rank != 0) return;
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   }
   __syncthreads();
-  ig -= gt;
-  ie -= eq;
-  for (int w = 0; w < warp; ++w) {
-    ig += s_scan[w];
-    ie += s_scan2[w];
+  key_hi = key_lo_c = big = 0;
+  for (int i = lane; i < nc * kWarps; i += 32) {
+    key_hi = max(key_hi, s_ends[i][0]);
+    key_lo_c = max(key_lo_c, s_ends[i][1]);
+    big = max(big, s_ends[i][2]);
   }
-  uint32_t pos = ig + min(ie, (uint32_t)left);
-  for (int i = i0; i < i1; ++i) {
-    const uint64_t k = s_key[i] & mask;
-    const bool take = k > prefix || (k == prefix && ie < (uint32_t)left);
-    ie += k == prefix;
-    if (take) out[a.sinks + pos++] = a.sinks + i;
+  key_hi = __reduce_max_sync(0xffffffffu, key_hi);
+  const uint32_t key_lo = ~__reduce_max_sync(0xffffffffu, key_lo_c);
+  big = __reduce_max_sync(0xffffffffu, big);
+  const float S = __uint_as_float(big) * l1;
+  bool exact = !(S > 8.7e-19f && S < 1.3e36f);   // 2^-60 .. 2^120, and not NaN
+
+  // 64-bit score of candidate i by one warp
+  auto score64 = [&](int page) -> uint64_t {
+    if (page < 0 || page >= a.num_pages) return 0ull;              // outside the pool: behind every other page
+    const uint8_t* b = bounds + (size_t)page * page_stride;
+    double s = 0.;
+    constexpr int kWords = kPageB / 128;         // 32-bit words per lane
+#pragma unroll
+    for (int w = 0; w < kWords; ++w) {
+      const uint32_t x = *reinterpret_cast<const uint32_t*>(b + (w * 32 + lane) * 4);
+      const int el = (w * 32 + lane) * (4 / kEl);
+      if constexpr (F8) {
+        double v[4];
+        fp8x4_to_f64(x, v);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) s = fma(s_q[el + q], v[q], s);
+      } else {
+        double v0, v1;
+        bf16x2_to_f64(x, v0, v1);
+        s = fma(s_q[el], v0, s);
+        s = fma(s_q[el + 1], v1, s);
+      }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    return sortable(s);
+  };
+
+  // warp w owns candidates [w * seg, (w + 1) * seg)
+  const int seg = (n + NT - 1) / NT * 32;
+  const int g0 = min(n, warp * seg), g1 = min(n, g0 + seg);
+  const uint32_t below = (1u << lane) - 1u;      // lanes before this one
+  if (!exact) {
+    // The need-th largest score lies in [lo, hi]: the bin of a histogram over the range of
+    // all scores, then over the edges of that bin, until few share one (scores above hi
+    // count in the top bin, which that score is not in).  A bin's edges are off by less than
+    // 2^-10 of its width; 2 E = 2^-17 S.
+    const float E2 = S * 7.62939453125e-06f;
+    float lo = from_sortable(key_lo), hi = from_sortable(key_hi);
+    uint32_t in_bin = (uint32_t)n;
+    while (in_bin > 8 && hi - lo > E2) {
+      const float width = (hi - lo) * (1.f / (kBins - 1)), inv = 1.f / width;
+      radix_count<NT>(sc, n, (uint32_t)need, [&](int i) -> int {
+        const float v = s_score[i];
+        return v > hi ? kBins - 1 : v >= lo ? min(kBins - 2, (int)((v - lo) * inv)) : -1;
+      });
+      in_bin = sc.in_bin;
+      const float l = lo + width * ((float)sc.border - 0x1p-10f), h = lo + width * ((float)(sc.border + 1) + 0x1p-10f);
+      lo = fmaxf(lo, l);
+      hi = fminf(hi, h);
+      __syncthreads();
+    }
+    lo -= E2;
+    hi += E2;
+    // list the pages that may go either way, count those above
+    uint32_t above = 0, listed_w = 0;
+#pragma unroll 4
+    for (int i = g0 + lane; i < g1; i += 32) {
+      const float v = s_score[i];
+      above += v > hi;
+      if (v >= lo && v <= hi) {
+        ++listed_w;
+        const uint32_t at = atomicAdd(&s_count, 1u);
+        if (at < kSelList) {
+          s_lidx[at] = i;
+          s_lval[at] = v;
+        }
+      }
+    }
+    above = __reduce_add_sync(0xffffffffu, above);
+    listed_w = __reduce_add_sync(0xffffffffu, listed_w);
+    if (lane == 0) {
+      s_cnt[0][warp] = above;
+      s_cnt[1][warp] = listed_w;
+    }
+    __syncthreads();
+    uint32_t take = (uint32_t)need;              // pages of the list to take: 1 .. listed
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) take -= s_cnt[0][w];
+    const uint32_t listed = s_count;
+    exact = listed > kSelList && listed > take;
+    if (!exact) {
+      if (listed > take) {
+        // the need-th largest score b itself, the pages that are surely above it, and those
+        // within 2 E of it: all of these are taken, or 64-bit scores tell them apart
+        const bool in = (uint32_t)tid < listed;
+        const float v = in ? s_lval[tid] : 0.f;
+        const int idx = in ? s_lidx[tid] : 0;
+        if (in) {
+          uint32_t more = 0, same = 0;
+          for (uint32_t j = 0; j < listed; ++j) {
+            more += s_lval[j] > v;
+            same += s_lval[j] == v;
+          }
+          if (more < take && more + same >= take) s_b = v;
+        }
+        __syncthreads();
+        const bool sure = in && v > s_b + E2, near = in && !sure && v >= s_b - E2;
+        const uint32_t sures = __syncthreads_count(sure), nears = __syncthreads_count(near);
+        bool taken = sure || near;
+        if (sures + nears > take) {
+          if (near) s_near[atomicAdd(&s_nears, 1u)] = tid;
+          __syncthreads();
+          for (uint32_t i = warp; i < nears; i += kWarps) {
+            const uint64_t k = score64(s_page[s_lidx[s_near[i]]]);
+            if (lane == 0) s_lkey[s_near[i]] = k;
+          }
+          __syncthreads();
+          if (near) {
+            const uint64_t k = s_lkey[tid];
+            uint32_t better = 0;
+            for (uint32_t j = 0; j < nears; ++j) {
+              const int o = s_near[j];
+              better += s_lkey[o] > k || (s_lkey[o] == k && s_lidx[o] < idx);
+            }
+            taken = better < take - sures;
+          }
+        }
+        if (in) {
+          s_score[idx] = taken ? INFINITY : -INFINITY;
+          if (!taken) atomicSub(&s_cnt[1][idx / seg], 1u);
+        }
+        __syncthreads();
+      }
+      uint32_t pos = (uint32_t)a.sinks;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) pos += w < warp ? s_cnt[0][w] + s_cnt[1][w] : 0u;
+#pragma unroll 4
+      for (int i0 = g0; i0 < g1; i0 += 32) {
+        const int i = i0 + lane;
+        const bool on = i < g1 && s_score[i] >= lo;
+        const uint32_t hit = __ballot_sync(0xffffffffu, on);
+        if (on) out[pos + __popc(hit & below)] = a.sinks + i;
+        pos += __popc(hit);
+      }
+      return;
+    }
+  }
+  // ---- 64-bit scores of all candidates
+  __syncthreads();
+  uint64_t top = 0, low_c = 0;
+  for (int i = warp; i < n; i += kWarps) {
+    const uint64_t k = score64(bt[i]);
+    if (lane == 0) s_key[i] = k;
+    top = max(top, k);
+    low_c = max(low_c, ~k);
+  }
+  if (lane == 0) {
+    sc.red[0][warp] = top;
+    sc.red[1][warp] = low_c;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    top = max(top, sc.red[0][w]);
+    low_c = max(low_c, sc.red[1][w]);
+  }
+  Border<uint64_t> b;
+  b.start(top, ~low_c, (uint32_t)need, n);
+  while (b.shift > 0 && b.in_bin != b.left) radix_pass<NT>(sc, n, [&](int i) { return s_key[i]; }, b);
+  // keys above the border's are taken, and of those on it the first `left`
+  uint32_t gt = 0, eq = 0;
+  for (int i = g0 + lane; i < g1; i += 32) {
+    const uint64_t k = s_key[i] & b.mask;
+    gt += k > b.prefix;
+    eq += k == b.prefix;
+  }
+  gt = __reduce_add_sync(0xffffffffu, gt);
+  eq = __reduce_add_sync(0xffffffffu, eq);
+  if (lane == 0) {
+    s_cnt[0][warp] = gt;
+    s_cnt[1][warp] = eq;
+  }
+  __syncthreads();
+  uint32_t ties = 0, pos = (uint32_t)a.sinks;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    pos += w < warp ? s_cnt[0][w] : 0u;
+    ties += w < warp ? s_cnt[1][w] : 0u;
+  }
+  pos += min(ties, b.left);
+  for (int i0 = g0; i0 < g1; i0 += 32) {
+    const int i = i0 + lane;
+    const uint64_t k = i < g1 ? s_key[i] & b.mask : 0ull;
+    const bool tie = i < g1 && k == b.prefix;
+    const uint32_t tie_hit = __ballot_sync(0xffffffffu, tie);
+    const bool on = i < g1 && (k > b.prefix || (tie && ties + __popc(tie_hit & below) < b.left));
+    const uint32_t hit = __ballot_sync(0xffffffffu, on);
+    if (on) out[pos + __popc(hit & below)] = a.sinks + i;
+    pos += __popc(hit);
+    ties += __popc(tie_hit);
   }
 }
 
-template <int D, bool F8>
-static void launch_select(const SelectArgs& a, cudaStream_t st) {
+template <int D, bool F8, int NT>
+static void launch_select(const SelectArgs& a, int nc, cudaStream_t st) {
   const size_t smem = (size_t)a.max_pages * sizeof(uint64_t);
-  auto kern = select_kernel<D, F8>;
-  if (smem > 40 * 1024) VRM_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  launch_kernel(kern, dim3(a.KH, a.T), dim3(kSelThreads), smem, st, a);
+  auto kern = select_kernel<D, F8, NT>;
+  if (smem > 32 * 1024) VRM_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  const dim3 grid(nc, a.KH, a.T);
+  if (nc > 1) launch_kernel_cluster(kern, grid, dim3(NT), dim3(nc, 1, 1), smem, st, a);
+  else launch_kernel(kern, grid, dim3(NT), smem, st, a);
 }
 
 void select_pages(const SelectArgs& in, cudaStream_t st) {
@@ -710,32 +1183,36 @@ void select_pages(const SelectArgs& in, cudaStream_t st) {
   SelectArgs a = in;
   a.err = error_word();
   VRM_REQUIRE(a.D == 64 || a.D == 128, "select_pages: head_dim must be 64 or 128");
-  VRM_REQUIRE(a.max_pages <= 24576, "select_pages: more than 24576 pages a sequence");
+  VRM_REQUIRE(a.max_pages <= kSelMaxPages, "select_pages: more than 24576 pages a sequence");
   VRM_REQUIRE(a.T <= 65535, "select_pages: too many query rows");
-  if (a.D == 128) a.f8 ? launch_select<128, true>(a, st) : launch_select<128, false>(a, st);
-  else a.f8 ? launch_select<64, true>(a, st) : launch_select<64, false>(a, st);
+  // Few rows: a cluster shares a row's candidates, as long as all CTAs fit two to an SM.
+  // Many: CTAs of 4 warps, four to an SM, so that one's choosing hides behind the others'
+  // reading.  B200, 32k tokens, D = 128, 8 kv heads (us): 1 row 22.9 / 16.4 / 13.0 / 11.7 with
+  // 1 / 2 / 4 / 8 CTAs, 16 rows 39.8 / 30.0 / 34.7 / 43.1; 8 against 4 warps: 32 rows of 16k
+  // tokens 27.0 / 38.7, 64 rows of fp8 bounds 64.5 / 58.1.
+  const long long rows = (long long)a.T * a.KH, fit = 2ll * device_sm_count();
+  int nc = 1;
+  while (nc < 8 && rows * nc * 2 <= fit) nc *= 2;
+  auto go = [&](auto d, auto f8) {
+    constexpr int D = decltype(d)::value;
+    constexpr bool F8 = decltype(f8)::value;
+    if (rows <= fit) launch_select<D, F8, 256>(a, nc, st);
+    else launch_select<D, F8, 128>(a, nc, st);
+  };
+  using D128 = std::integral_constant<int, 128>;
+  using D64 = std::integral_constant<int, 64>;
+  if (a.D == 128) a.f8 ? go(D128{}, std::true_type{}) : go(D128{}, std::false_type{});
+  else a.f8 ? go(D64{}, std::true_type{}) : go(D64{}, std::false_type{});
   VRM_CUDA_CHECK(cudaGetLastError());
 }
 
 // ================================================================ attention over selected pages
 namespace {
 
-__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                        uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-      "{%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
-}
-__device__ __forceinline__ uint32_t fp8x2_to_half2(uint32_t v) {
-  __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)v, __NV_E4M3);
-  return (uint32_t)h.x | ((uint32_t)h.y << 16);
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   uint32_t r;
@@ -763,63 +1240,65 @@ struct Frag {
   static constexpr int kCodeB = FMT == kFmtQ4 ? D / 2 : kRowB;      // bytes of values in a row
   static constexpr int kKB = kCodeB / 4;                            // bytes of a row per lane, K
   static constexpr int kVB = kCodeB / 8;                            // V
-  static constexpr int kKW = kKB / 4, kVW = kVB / 4;                // 32-bit words
-  uint32_t k[2][kKW], v[4][kVW];
+  static constexpr int kPK = kKB < 16 ? kKB : 16, kPV = kVB < 16 ? kVB : 16;   // bytes of a piece
+  uint32_t k[2][kKB / 4], v[4][kVB / 4];
   uint32_t ks[FMT == kFmtQ4 ? 2 : 1], vs[FMT == kFmtQ4 ? 4 : 1];    // {scale, min}
 
-  template <int W>
-  static __device__ __forceinline__ void piece(uint32_t* dst, const uint8_t* p) {
-    if constexpr (W == 4) {
-      const uint4 x = ld_stream16(p);
-      dst[0] = x.x, dst[1] = x.y, dst[2] = x.z, dst[3] = x.w;
-    } else if constexpr (W == 2) {
-      const uint2 x = ld_stream8(p);
-      dst[0] = x.x, dst[1] = x.y;
-    } else {
-      dst[0] = ld_stream4(p);
-    }
-  }
-  // rows >= `rows` (behind the context) are not read and count as zeros.  Four-bit rows
-  // are 8-byte aligned only (16 for D = 128).
-  __device__ __forceinline__ void load_k(const uint8_t* kp, int rows, int g, int c) {
-    constexpr int W = kKW < 4 ? kKW : 4;
+  template <bool ALL>
+  __device__ __forceinline__ void get_k(const uint8_t* kp, int rows, int g, int c) {
+    const uint8_t* p0 = kp + g * kRowB + c * kPK;
+    const uint8_t* s0 = kp + g * kRowB + D / 2 + (D == 128 ? c : c / 2) * 4;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int r = g + 8 * h;
-      const uint8_t* p = kp + r * kRowB;
-      const bool on = r < rows;
+      if (ALL || g + 8 * h < rows) {
 #pragma unroll
-      for (int i = 0; i < kKW; ++i) k[h][i] = 0u;
-      if (FMT == kFmtQ4) ks[FMT == kFmtQ4 ? h : 0] = 0u;
-      if (on) {
+        for (int i = 0; i < kKB / kPK; ++i) ld_stream<kPK>(&k[h][i * kPK / 4], p0 + h * 8 * kRowB + i * 4 * kPK);
+        if constexpr (FMT == kFmtQ4) ld_stream<4>(&ks[h], s0 + h * 8 * kRowB);
+      } else {
 #pragma unroll
-        for (int i = 0; i < kKW / W; ++i) piece<W>(&k[h][i * W], p + (i * 4 + c) * (W * 4));
-        if constexpr (FMT == kFmtQ4) ks[h] = ld_stream4(p + D / 2 + (D == 128 ? c : c / 2) * 4);
+        for (int i = 0; i < kKB / 4; ++i) k[h][i] = 0u;
+        if constexpr (FMT == kFmtQ4) ks[h] = 0u;
       }
     }
   }
-  __device__ __forceinline__ void load_v(const uint8_t* vp, int rows, int g, int c) {
-    constexpr int W = kVW < 4 ? kVW : 4;
+  template <bool ALL>
+  __device__ __forceinline__ void get_v(const uint8_t* vp, int rows, int g, int c) {
+    const uint8_t* p0 = vp + 2 * c * kRowB + g * kPV;
+    const uint8_t* s0 = vp + 2 * c * kRowB + D / 2 + (D == 128 ? g / 2 : g / 4) * 4;
 #pragma unroll
     for (int h = 0; h < 4; ++h) {
-      const int r = 2 * c + (h & 1) + 8 * (h >> 1);
-      const uint8_t* p = vp + r * kRowB;
-      const bool on = r < rows;
+      const int r = (h & 1) + 8 * (h >> 1);
+      if (ALL || 2 * c + r < rows) {
 #pragma unroll
-      for (int i = 0; i < kVW; ++i) v[h][i] = 0u;
-      if (FMT == kFmtQ4) vs[FMT == kFmtQ4 ? h : 0] = 0u;
-      if (on) {
+        for (int i = 0; i < kVB / kPV; ++i) ld_stream<kPV>(&v[h][i * kPV / 4], p0 + r * kRowB + i * 8 * kPV);
+        if constexpr (FMT == kFmtQ4) ld_stream<4>(&vs[h], s0 + r * kRowB);
+      } else {
 #pragma unroll
-        for (int i = 0; i < kVW / W; ++i) piece<W>(&v[h][i * W], p + (i * 8 + g) * (W * 4));
-        if constexpr (FMT == kFmtQ4) vs[h] = ld_stream4(p + D / 2 + (D == 128 ? g / 2 : g / 4) * 4);
+        for (int i = 0; i < kVB / 4; ++i) v[h][i] = 0u;
+        if constexpr (FMT == kFmtQ4) vs[h] = 0u;
       }
     }
+  }
+  // rows >= `rows` (behind the context) are not read and count as zeros
+  __device__ __forceinline__ void load_k(const uint8_t* kp, int rows, int g, int c) {
+    if (rows == kPageTok) get_k<true>(kp, rows, g, c);
+    else get_k<false>(kp, rows, g, c);
+  }
+  __device__ __forceinline__ void load_v(const uint8_t* vp, int rows, int g, int c) {
+    if (rows == kPageTok) get_v<true>(vp, rows, g, c);
+    else get_v<false>(vp, rows, g, c);
   }
   // first of the four dims that step s of the score product takes from lane c
   static __device__ __forceinline__ int k_dim(int s, int c) {
     if constexpr (FMT == kFmtBf16) return (c + 4 * (s / 2)) * 8 + 4 * (s % 2);
     else if constexpr (FMT == kFmtFp8) return (c + 4 * (s / 4)) * 16 + 4 * (s % 4);
     else return c * (D / 4) + 4 * s;
+  }
+  // q's fragment of step s from the eight dims 8 (s / 2) .. of lane c's four-bit piece: the
+  // pairs of a code word that one mask takes out are (0, 4), (1, 5) | (2, 6), (3, 7)
+  static __device__ __forceinline__ uint2 q4_pairs(const uint2& lo, const uint2& hi, int s) {
+    const uint32_t a = s % 2 ? lo.y : lo.x, b = s % 2 ? hi.y : hi.x;
+    return make_uint2(__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632));
   }
   // A fragment of step s: dims k_dim .. + 1 of rows g, g + 8, then k_dim + 2 .. + 3
   __device__ __forceinline__ void k_frag(int s, uint32_t (&a)[4]) const {
@@ -837,9 +1316,9 @@ struct Frag {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const uint32_t s2 = __byte_perm(ks[h], 0, 0x1010), m2 = __byte_perm(ks[h], 0, 0x3232);
-        const uint32_t w = k[h][s / 2] >> (16 * (s % 2));       // two code bytes: four dims
-        a[h] = codes_to_half2((w & 0xFu) | ((w & 0xF0u) << 12), s2, m2);
-        a[2 + h] = codes_to_half2(((w >> 8) & 0xFu) | ((w & 0xF000u) << 4), s2, m2);
+        const uint32_t w = k[h][s / 2] >> (8 * (s % 2));        // dims 0 and 4, 1 and 5 of it, or 2 and 6, 3 and 7
+        a[h] = codes_to_half2(w, s2, m2);
+        a[2 + h] = codes_to_half2(w >> 4, s2, m2);
       }
     }
   }
@@ -857,13 +1336,13 @@ struct Frag {
         a[q] = __byte_perm(v[t0][w], v[t0 + 1][w], e % 2 ? 0x7632 : 0x5410);
       } else if constexpr (FMT == kFmtFp8) {
         const int dim = (D / 16) * hi + e;
-        const uint32_t x = __byte_perm(v[t0][dim / 4], v[t0 + 1][dim / 4], 0x40 + 0x11 * (dim % 4));
-        a[q] = fp8x2_to_half2(x & 0xffffu);
+        const uint32_t x = __byte_perm(v[t0][dim / 4], v[t0 + 1][dim / 4], dim % 4 < 2 ? 0x5140 : 0x7362);
+        a[q] = fp8x2_to_half2(dim % 2 ? x >> 16 : x);
       } else {
-        const int dim = (D / 16) * hi + e, b = dim / 2;
-        const uint32_t x = __byte_perm(v[t0][b / 4], v[t0 + 1][b / 4], 0x0400 + 0x0101 * (b % 4));
+        const int dim = (D / 16) * hi + e;
+        const uint32_t x = __byte_perm(v[t0][dim / 8], v[t0 + 1][dim / 8], dim % 8 < 4 ? 0x5410 : 0x7632);
         const uint32_t s2 = __byte_perm(vs[t0], vs[t0 + 1], 0x5410), m2 = __byte_perm(vs[t0], vs[t0 + 1], 0x7632);
-        a[q] = codes_to_half2(dim % 2 ? x >> 4 : x, s2, m2);
+        a[q] = codes_to_half2(x >> (4 * (dim % 4)), s2, m2);
       }
     }
   }
@@ -871,31 +1350,47 @@ struct Frag {
 
 }  // namespace
 
+// Pages a warp takes at a time and CTAs an SM holds.  Pages of 8 KB (bf16, D = 128): two
+// at a time in 244 registers, so that each of the SM's 8 warps has 16 KB under way; narrower
+// pages cost more arithmetic a byte, and 16 warps with one page each run better (B200, us:
+// 32 rows of bf16 43.9 against 77.9 with one page and 4 CTAs; 128 rows of fp8 92.0 against
+// 96.0 with four pages and 2 CTAs, four-bit 64 rows 58.1 against 59.4).
+template <int D, int FMT>
+struct AttendShape {
+  static constexpr bool kWide = FMT == kFmtBf16 && D == 128;
+  static constexpr int kTurn = kWide ? 2 : 1, kCtas = kWide ? 2 : 4;
+};
+
 // One CTA of 4 warps per (kv head, query row, split); the warps of all splits take the
 // row's pages in turn.  Scores are computed transposed, S^T = K Q^T: a page's 16 tokens
-// fill the MMA rows and the group's (<= 8) heads its columns; O^T = V^T P^T likewise.
-// Splits are the CTAs of one cluster and merge through distributed shared memory.
+// fill the MMA rows and the group's (<= 8) heads its columns; O^T = V^T P^T likewise.  A
+// warp requests its next page's K as soon as the scores have used the present one's, and V
+// after the outputs, so that loads are in flight all the time.  Splits are the CTAs of one
+// cluster: each pushes its partial outputs to the CTAs that finish them, through
+// distributed shared memory.
 template <int D, int FMT>
-__global__ void __launch_bounds__(128) attend_kernel(AttendArgs P) {
+__global__ void __launch_bounds__(128, AttendShape<D, FMT>::kCtas) attend_kernel(AttendArgs P) {
   using F = Frag<D, FMT>;
+  constexpr int kTurn = AttendShape<D, FMT>::kTurn;
   constexpr int kSteps = D / 16;
-  constexpr int kOS = D + 4;
+  constexpr int kOS = D + 1;                           // odd: the transposed stores meet in two lanes a bank
   __shared__ float s_m[4][8], s_l[4][8];
   __shared__ float s_o[4 * 8 * kOS];
-  __shared__ float s_co[8 * D], s_cm[8], s_cl[8];
+  __shared__ float s_in[8 * D], s_ml[8][2][8];         // what the splits pushed: [split][head][dim], [split][m, l][head]
+  __shared__ float s_w[8][8], s_max[8], s_sum[8];      // weights of the parts of a merge, their maximum and sum
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
   pdl_launch();
   pdl_wait();
   const int kvh = blockIdx.x, t = blockIdx.y, split = blockIdx.z, nsplit = gridDim.z;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
   const int G = P.G, KH = P.KH;
-  RowOf row;
-  if (!find_row(t, P.cu_q, P.context_lens, P.B, row)) return;      // the same for the whole cluster
+  const int stride = 4 * nsplit;
   const int* list = P.pages + ((size_t)t * KH + kvh) * P.S;
-  const int* bt = P.block_tables + (size_t)row.seq * P.bt_stride;
-  const size_t head_b = (size_t)kPageTok * F::kRowB;
-  const size_t page_b = (size_t)P.num_layers * 2 * KH * head_b;
-  const uint8_t* pool = reinterpret_cast<const uint8_t*>(P.cache) + ((size_t)P.layer * 2 * KH + kvh) * head_b;
+  // 32 list entries of this warp, one a lane; the first are requested beside the row's length
+  auto entry = [&](int base) -> int { return base + lane * stride < P.S ? list[base + lane * stride] : -1; };
+  int lp = entry(split * 4 + warp);
 
   // Q as the B operand: step s, lane (g, c) holds dims k_dim(s, c) .. + 3 of head g
   uint2 qb[kSteps];
@@ -910,80 +1405,126 @@ __global__ void __launch_bounds__(128) attend_kernel(AttendArgs P) {
     scale_log2 *= P.kv_scale[(P.layer * 2 + 0) * KH + kvh];
     v_scale = P.kv_scale[(P.layer * 2 + 1) * KH + kvh];
   }
-  if constexpr (FMT != kFmtBf16) {
-    // f16 operands: q times the power of two that brings its largest value to [1, 2)
-    float mx = 0.f;
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s)
-      mx = fmaxf(mx, fmaxf(fmaxf(fabsf(bf16_lo(qb[s].x)), fabsf(bf16_hi(qb[s].x))),
-                           fmaxf(fabsf(bf16_lo(qb[s].y)), fabsf(bf16_hi(qb[s].y)))));
-    mx = warp_max(mx);
-    const int e = (int)(__float_as_uint(mx) >> 23);
-    float f = 1.f;
-    if (e > 1 && e < 253) {
-      f = __uint_as_float((uint32_t)(254 - e) << 23);
-      scale_log2 *= __uint_as_float((uint32_t)e << 23);
-    }
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      qb[s].x = pack_half2(bf16_lo(qb[s].x) * f, bf16_hi(qb[s].x) * f);
-      qb[s].y = pack_half2(bf16_lo(qb[s].y) * f, bf16_hi(qb[s].y) * f);
-    }
-  }
+  RowOf row;
+  if (!find_row(t, P.cu_q, P.context_lens, P.B, row)) return;      // the same for the whole cluster
+  if (nsplit > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // this CTA runs
+  const int* bt = P.block_tables + (size_t)row.seq * P.bt_stride;
+  const size_t head_b = (size_t)kPageTok * F::kRowB;
+  const size_t page_b = (size_t)P.num_layers * 2 * KH * head_b;
+  const uint8_t* pool = reinterpret_cast<const uint8_t*>(P.cache) + ((size_t)P.layer * 2 * KH + kvh) * head_b;
 
   float o[kSteps][4];
 #pragma unroll
   for (int i = 0; i < kSteps; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
   float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
-  bool seen = false;
+  bool seen = false, q_ready = FMT == kFmtBf16;
 
-  const int stride = 4 * nsplit;
   for (int base = split * 4 + warp; base < P.S; base += 32 * stride) {
-    // 32 list entries of this warp: logical page, physical page, tokens to read
-    const int i = base + lane * stride;
-    const int lp = i < P.S ? list[i] : -1;
+    // physical page and tokens to read of the lane's entry
     int phys = 0, rows = 0;
     if (lp >= 0 && lp < P.max_pages && (long long)lp * kPageTok < row.n) {
       phys = bt[lp];
       if (phys >= 0 && phys < P.num_pages) rows = min(kPageTok, row.n - lp * kPageTok);
       else report_error(P.err, kErrBounds);
     }
-    const int cnt = min(32, (P.S - base + stride - 1) / stride);
-    for (int j = 0; j < cnt; ++j) {
-      const int r = __shfl_sync(0xffffffffu, rows, j);
-      const int ph = __shfl_sync(0xffffffffu, phys, j);
-      if (r == 0) continue;
-      seen = true;
-      const uint8_t* kp = pool + (size_t)ph * page_b;
-      F f;
-      f.load_k(kp, r, g, c);
-      f.load_v(kp + (size_t)KH * head_b, r, g, c);
-      float sc[4] = {0.f, 0.f, 0.f, 0.f};
+    lp = entry(base + 32 * stride);
+    uint32_t todo = __ballot_sync(0xffffffffu, rows > 0);
+    if (todo == 0) continue;
+    seen = true;
+    // the pages of a turn: kTurn set bits of todo (rows 0: none left)
+    F f[kTurn];
+    const uint8_t* kp[kTurn];
+    int r[kTurn];
+    auto take = [&] {
+#pragma unroll
+      for (int q = 0; q < kTurn; ++q) {
+        const int j = todo ? __ffs(todo) - 1 : 0;
+        const int rj = __shfl_sync(0xffffffffu, rows, j);
+        kp[q] = pool + (size_t)__shfl_sync(0xffffffffu, phys, j) * page_b;
+        r[q] = todo ? rj : 0;
+        todo &= todo - 1;
+      }
+    };
+    take();
+#pragma unroll
+    for (int q = 0; q < kTurn; ++q) f[q].load_k(kp[q], r[q], g, c);
+#pragma unroll
+    for (int q = 0; q < kTurn; ++q) f[q].load_v(kp[q] + (size_t)KH * head_b, r[q], g, c);
+    if (!q_ready) {
+      // f16 operands: q times the power of two that brings its largest value to [1, 2)
+      float mx = 0.f;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
+        mx = fmaxf(mx, fmaxf(fmaxf(fabsf(bf16_lo(qb[s].x)), fabsf(bf16_hi(qb[s].x))),
+                             fmaxf(fabsf(bf16_lo(qb[s].y)), fabsf(bf16_hi(qb[s].y)))));
+      mx = warp_max(mx);
+      const int e = (int)(__float_as_uint(mx) >> 23);
+      float x = 1.f;
+      if (e > 1 && e < 253) {
+        x = __uint_as_float((uint32_t)(254 - e) << 23);
+        scale_log2 *= __uint_as_float((uint32_t)e << 23);
+      }
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
-        uint32_t a[4];
-        f.k_frag(s, a);
-        if constexpr (FMT == kFmtBf16) mma_bf16_16816(sc, a[0], a[1], a[2], a[3], qb[s].x, qb[s].y);
-        else mma_f16(sc, a[0], a[1], a[2], a[3], qb[s].x, qb[s].y);
+        qb[s].x = pack_half2(bf16_lo(qb[s].x) * x, bf16_hi(qb[s].x) * x);
+        qb[s].y = pack_half2(bf16_lo(qb[s].y) * x, bf16_hi(qb[s].y) * x);
       }
-      // sc[0] = (token g, head 2c), [1] = (g, 2c + 1), [2] = (g + 8, 2c), [3] = (g + 8, 2c + 1)
-      float x[4] = {sc[0] * scale_log2, sc[1] * scale_log2, sc[2] * scale_log2, sc[3] * scale_log2};
-      if (g >= r) x[0] = x[1] = -INFINITY;
-      if (g + 8 >= r) x[2] = x[3] = -INFINITY;
-      float mx[2] = {fmaxf(x[0], x[2]), fmaxf(x[1], x[3])};
-      float alpha[2], pr[4];
+      if constexpr (FMT == kFmtQ4) {
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        mx[q] = fmaxf(mx[q], __shfl_xor_sync(0xffffffffu, mx[q], 4));
-        mx[q] = fmaxf(mx[q], __shfl_xor_sync(0xffffffffu, mx[q], 8));
-        mx[q] = fmaxf(mx[q], __shfl_xor_sync(0xffffffffu, mx[q], 16));
-        const float m_new = fmaxf(m_run[q], mx[q]);
+        for (int s = 0; s < kSteps; s += 2) {
+          const uint2 lo = qb[s], hi = qb[s + 1];
+          qb[s] = F::q4_pairs(lo, hi, 0);
+          qb[s + 1] = F::q4_pairs(lo, hi, 1);
+        }
+      }
+      q_ready = true;
+    }
+    bool more = true;
+    while (more) {
+      int r_now[kTurn];
+#pragma unroll
+      for (int q = 0; q < kTurn; ++q) r_now[q] = r[q];
+      more = todo != 0;
+      if (more) take();
+      float x[kTurn][4], mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int q = 0; q < kTurn; ++q) {
+        float sc[4] = {0.f, 0.f, 0.f, 0.f}, sd[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+          uint32_t a[4];
+          f[q].k_frag(s, a);
+          if constexpr (FMT == kFmtBf16) mma_bf16_16816(s % 2 ? sd : sc, a[0], a[1], a[2], a[3], qb[s].x, qb[s].y);
+          else mma_f16(s % 2 ? sd : sc, a[0], a[1], a[2], a[3], qb[s].x, qb[s].y);
+        }
+        if (more) f[q].load_k(kp[q], r[q], g, c);
+        // sc[0] = (token g, head 2c), [1] = (g, 2c + 1), [2] = (g + 8, 2c), [3] = (g + 8, 2c + 1)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[q][i] = (sc[i] + sd[i]) * scale_log2;
+        if (r_now[q] != kPageTok) {
+          if (g >= r_now[q]) x[q][0] = x[q][1] = -INFINITY;
+          if (g + 8 >= r_now[q]) x[q][2] = x[q][3] = -INFINITY;
+        }
+        mx[0] = fmaxf(mx[0], fmaxf(x[q][0], x[q][2]));
+        mx[1] = fmaxf(mx[1], fmaxf(x[q][1], x[q][3]));
+      }
+      float alpha[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 4));
+        mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 8));
+        mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 16));
+        const float m_new = fmaxf(m_run[h], mx[h]);
         const float m_use = m_new == -INFINITY ? 0.f : m_new;
-        alpha[q] = exp2f(m_run[q] - m_use);
-        pr[q] = exp2f(x[q] - m_use);
-        pr[2 + q] = exp2f(x[2 + q] - m_use);
-        m_run[q] = m_new;
-        l_run[q] = l_run[q] * alpha[q] + (pr[q] + pr[2 + q]);
+        alpha[h] = ex2(m_run[h] - m_use);
+        m_run[h] = m_new;
+        l_run[h] *= alpha[h];
+#pragma unroll
+        for (int q = 0; q < kTurn; ++q) {
+          x[q][h] = ex2(x[q][h] - m_use);
+          x[q][2 + h] = ex2(x[q][2 + h] - m_use);
+          l_run[h] += x[q][h] + x[q][2 + h];
+        }
       }
 #pragma unroll
       for (int e = 0; e < kSteps; ++e) {
@@ -992,20 +1533,24 @@ __global__ void __launch_bounds__(128) attend_kernel(AttendArgs P) {
         o[e][2] *= alpha[0];
         o[e][3] *= alpha[1];
       }
-      uint32_t pb0, pb1;
-      if constexpr (FMT == kFmtBf16) {
-        pb0 = transpose8x8(pack_bf16x2(pr[0], pr[1]));
-        pb1 = transpose8x8(pack_bf16x2(pr[2], pr[3]));
-      } else {
-        pb0 = transpose8x8(pack_half2(pr[0], pr[1]));
-        pb1 = transpose8x8(pack_half2(pr[2], pr[3]));
-      }
 #pragma unroll
-      for (int e = 0; e < kSteps; ++e) {
-        uint32_t a[4];
-        f.v_frag(e, a);
-        if constexpr (FMT == kFmtBf16) mma_bf16_16816(o[e], a[0], a[1], a[2], a[3], pb0, pb1);
-        else mma_f16(o[e], a[0], a[1], a[2], a[3], pb0, pb1);
+      for (int q = 0; q < kTurn; ++q) {
+        uint32_t pb0, pb1;
+        if constexpr (FMT == kFmtBf16) {
+          pb0 = transpose8x8(pack_bf16x2(x[q][0], x[q][1]));
+          pb1 = transpose8x8(pack_bf16x2(x[q][2], x[q][3]));
+        } else {
+          pb0 = transpose8x8(pack_half2(x[q][0], x[q][1]));
+          pb1 = transpose8x8(pack_half2(x[q][2], x[q][3]));
+        }
+#pragma unroll
+        for (int e = 0; e < kSteps; ++e) {
+          uint32_t a[4];
+          f[q].v_frag(e, a);
+          if constexpr (FMT == kFmtBf16) mma_bf16_16816(o[e], a[0], a[1], a[2], a[3], pb0, pb1);
+          else mma_f16(o[e], a[0], a[1], a[2], a[3], pb0, pb1);
+        }
+        if (more) f[q].load_v(kp[q] + (size_t)KH * head_b, r[q], g, c);
       }
     }
   }
@@ -1034,59 +1579,89 @@ __global__ void __launch_bounds__(128) attend_kernel(AttendArgs P) {
     r0[kOS + F::v_dim(e, g, 1)] = o[e][3];
   }
   __syncthreads();
+  // weights of up to 8 partial sums with maxima m(w, h) and sums l(w, h), by one warp: lane
+  // (w % 4, h) has parts w and w + 4
+  auto weigh = [&](int parts, auto m, auto l) {
+    if (warp != 0) return;
+    const int h = lane & 7, w = lane >> 3;
+    const float m0 = w < parts ? m(w, h) : -INFINITY, m1 = w + 4 < parts ? m(w + 4, h) : -INFINITY;
+    const float l0 = w < parts ? l(w, h) : 0.f, l1 = w + 4 < parts ? l(w + 4, h) : 0.f;
+    float M = fmaxf(m0, m1);
+    M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, 8));
+    M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, 16));
+    const float f0 = m0 == -INFINITY ? 0.f : ex2(m0 - M), f1 = m1 == -INFINITY ? 0.f : ex2(m1 - M);
+    // no score above -inf anywhere: the sums are 0, or NaN
+    float L = M == -INFINITY ? l0 + l1 : (f0 == 0.f ? 0.f : f0 * l0) + (f1 == 0.f ? 0.f : f1 * l1);
+    L += __shfl_xor_sync(0xffffffffu, L, 8);
+    L += __shfl_xor_sync(0xffffffffu, L, 16);
+    s_w[w][h] = f0;
+    s_w[w + 4][h] = f1;
+    if (w == 0) {
+      s_max[h] = M;
+      s_sum[h] = L;
+    }
+    __syncwarp();
+  };
+  weigh(4, [&](int w, int h) { return s_m[w][h]; }, [&](int w, int h) { return s_l[w][h]; });
+  if (nsplit > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");      // the others run
+  if (nsplit > 1 && warp == 0) {
+    for (int q = lane >> 3; q < nsplit; q += 4) {
+      float* ml = cluster.map_shared_rank(&s_ml[0][0][0], q) + split * 16 + (lane & 7);
+      ml[0] = s_max[lane & 7];
+      ml[8] = s_sum[lane & 7];
+    }
+  }
+  __syncthreads();
   __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(P.out) + (size_t)t * P.ld_o + (size_t)kvh * G * D;
-  for (int idx = threadIdx.x; idx < G * D; idx += 128) {
-    const int h = idx / D, d = idx % D;
-    float M = fmaxf(fmaxf(s_m[0][h], s_m[1][h]), fmaxf(s_m[2][h], s_m[3][h]));
-    float L = 0.f, acc = 0.f;
+  // thread: dims d, d + 1 of heads h0, h0 + 256 / D ..; a split finishes D / nsplit dims of every head
+  const int d = 2 * (threadIdx.x % (D / 2)), h0 = threadIdx.x / (D / 2);
+  const int own = D / nsplit;
+  float* there = nsplit > 1 ? cluster.map_shared_rank(s_in, d / own) + split * 8 * own + d % own : nullptr;
+  for (int h = h0; h < G; h += 256 / D) {
+    float x = 0.f, y = 0.f;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      if (M == -INFINITY) {
-        L += s_l[w][h];                                    // 0, or NaN
-      } else if (s_m[w][h] != -INFINITY) {
-        const float f = exp2f(s_m[w][h] - M);
-        L += s_l[w][h] * f;
-        acc += s_o[(w * 8 + h) * kOS + d] * f;
+      const float f = s_w[w][h];
+      if (f != 0.f) {
+        x += f * s_o[(w * 8 + h) * kOS + d];
+        y += f * s_o[(w * 8 + h) * kOS + d + 1];
       }
     }
     if (nsplit == 1) {
-      out[idx] = __float2bfloat16(L == 0.f ? 0.f : acc / L * v_scale);
+      const float L = s_sum[h];
+      *reinterpret_cast<uint32_t*>(out + h * D + d) =
+          L == 0.f ? 0u : pack_bf16x2(x / L * v_scale, y / L * v_scale);
     } else {
-      s_co[idx] = acc;
-      if (d == 0) {
-        s_cm[h] = M;
-        s_cl[h] = L;
-      }
+      there[h * own] = x;
+      there[h * own + 1] = y;
     }
   }
   if (nsplit == 1) return;
-  namespace cg = cooperative_groups;
-  cg::cluster_group cluster = cg::this_cluster();
   cluster.sync();
-  const int n = G * D, per = (n + nsplit - 1) / nsplit;
-  const int i0 = split * per, i1 = min(n, i0 + per);
-  for (int idx = i0 + threadIdx.x; idx < i1; idx += 128) {
-    const int h = idx / D;
-    float M = -INFINITY;
-    for (int q = 0; q < nsplit; ++q) M = fmaxf(M, cluster.map_shared_rank(s_cm, q)[h]);
-    float L = 0.f, acc = 0.f;
-    for (int q = 0; q < nsplit; ++q) {
-      const float mq = cluster.map_shared_rank(s_cm, q)[h], lq = cluster.map_shared_rank(s_cl, q)[h];
-      if (M == -INFINITY) {
-        L += lq;
-      } else if (mq != -INFINITY) {
-        const float w = exp2f(mq - M);
-        L += w * lq;
-        acc += w * cluster.map_shared_rank(s_co, q)[idx];
-      }
+  weigh(nsplit, [&](int w, int h) { return s_ml[w][0][h]; }, [&](int w, int h) { return s_ml[w][1][h]; });
+  __syncthreads();
+  for (int i = threadIdx.x; i < G * own; i += 128) {
+    const int h = i / own;
+    float x = 0.f;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const float f = q < nsplit ? s_w[q][h] : 0.f;
+      if (f != 0.f) x += f * s_in[q * 8 * own + i];
     }
-    out[idx] = __float2bfloat16(L == 0.f ? 0.f : acc / L * v_scale);
+    const float L = s_sum[h];
+    out[h * D + split * own + i % own] = __float2bfloat16(L == 0.f ? 0.f : x / L * v_scale);
   }
-  cluster.sync();     // peers' shared memory stays valid until every CTA has read it
 }
 
 template <int D, int FMT>
-static void launch_attend(const AttendArgs& a, int splits, cudaStream_t st) {
+static void launch_attend(const AttendArgs& a, cudaStream_t st) {
+  // as many splits as keep all CTAs resident at once and leave every warp two pages: more
+  // CTAs than that queue, and each costs its start and its merge again (B200, us, splits
+  // 1 / 2 / 8: 1 row of bf16 25.0 / 16.4 / 8.7, 16 rows 35.9 / 26.1 / 46.8, 64 rows 83.8 / 99.6 / 156.7)
+  int splits = 1;
+  while (splits < 8 && (long long)a.T * a.KH * splits * 2 <= (long long)AttendShape<D, FMT>::kCtas * device_sm_count() &&
+         a.S >= 16 * splits)
+    splits *= 2;
   const dim3 grid(a.KH, a.T, splits);
   if (splits > 1) launch_kernel_cluster(attend_kernel<D, FMT>, grid, dim3(128), dim3(1, 1, splits), 0, st, a);
   else launch_kernel(attend_kernel<D, FMT>, grid, dim3(128), 0, st, a);
@@ -1099,13 +1674,11 @@ void paged_attention_selected(const AttendArgs& in, cudaStream_t st) {
   VRM_REQUIRE(a.D == 64 || a.D == 128, "paged_attention_selected: head_dim must be 64 or 128");
   VRM_REQUIRE(a.G >= 1 && a.G <= 8, "paged_attention_selected: GQA group must be <= 8 heads");
   VRM_REQUIRE(a.T <= 65535, "paged_attention_selected: too many query rows");
-  int splits = 1;
-  while (splits < 8 && (long long)a.T * a.KH * splits * 2 <= 2ll * device_sm_count() && a.S >= 8 * splits) splits *= 2;
   auto go = [&](auto d) {
     constexpr int D = decltype(d)::value;
-    if (a.fmt == kFmtQ4) launch_attend<D, kFmtQ4>(a, splits, st);
-    else if (a.fmt == kFmtFp8) launch_attend<D, kFmtFp8>(a, splits, st);
-    else launch_attend<D, kFmtBf16>(a, splits, st);
+    if (a.fmt == kFmtQ4) launch_attend<D, kFmtQ4>(a, st);
+    else if (a.fmt == kFmtFp8) launch_attend<D, kFmtFp8>(a, st);
+    else launch_attend<D, kFmtBf16>(a, st);
   };
   if (a.D == 128) go(std::integral_constant<int, 128>{});
   else go(std::integral_constant<int, 64>{});

@@ -396,8 +396,8 @@ void check_rows16(const Tensor& t, const char* name) {
 
 // key bounds [pages, layers, KH, 2, D]: bf16, or e4m3 (of fp8 pages)
 void check_bounds(const Tensor& b, const char* op) {
-  TORCH_CHECK(b.is_cuda() && b.dim() == 5 && b.is_contiguous() && b.size(3) == 2, op,
-              ": key_bounds must be a contiguous [pages, layers, kv_heads, 2, head_dim] CUDA tensor");
+  TORCH_CHECK(b.is_cuda() && b.dim() == 5 && b.is_contiguous() && b.size(3) == 2 && b.numel() > 0, op,
+              ": key_bounds must be a non-empty contiguous [pages, layers, kv_heads, 2, head_dim] CUDA tensor");
   TORCH_CHECK(b.scalar_type() == torch::kBFloat16 || b.scalar_type() == torch::kFloat8_e4m3fn, op,
               ": key_bounds must be bf16 or fp8");
   TORCH_CHECK(reinterpret_cast<uintptr_t>(b.data_ptr()) % 16 == 0, op, ": key_bounds must be 16-byte aligned");

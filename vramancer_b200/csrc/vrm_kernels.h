@@ -446,7 +446,7 @@ struct AppendArgs {
   void* bounds = nullptr;              // key bounds, or null
   void* q_out = nullptr;               // bf16, token t head h at q_out + t * ld_out + h * D
   int64_t ld_out = 0;
-  int heads_per_group = 0, q_groups = 0, v_groups = 0;   // set by the launcher
+  int k_tile = 0, heads_per_group = 0, q_groups = 0, v_groups = 0;   // set by the launcher
   uint32_t* err = nullptr;             // error word (set by the launcher)
 };
 void qk_norm_rope_kv_write(const AppendArgs& a, cudaStream_t stream);
