@@ -54,6 +54,8 @@ def build_parser() -> argparse.ArgumentParser:
     r.add_argument("--backend", default="auto")
     r.add_argument("--gpus", type=int, default=None)
     r.add_argument("--quantization", "-q", default=None, choices=QUANT_CHOICES)
+    r.add_argument("--sparse-pages", type=int, default=0,
+                   help="block-sparse decode: 16-token KV pages a token reads per layer and kv head (0: all)")
     r.add_argument("--num-layers", type=int, default=None, help=argparse.SUPPRESS)
 
     s = sub.add_parser("serve", help="OpenAI-compatible API server")
@@ -65,6 +67,8 @@ def build_parser() -> argparse.ArgumentParser:
     s.add_argument("--host", default="0.0.0.0")
     s.add_argument("--port", type=int, default=5030)
     s.add_argument("--quantization", "-q", default=None, choices=QUANT_CHOICES)
+    s.add_argument("--sparse-pages", type=int, default=0,
+                   help="block-sparse decode: 16-token KV pages a token reads per layer and kv head (0: all)")
     s.add_argument("--no-cluster", dest="cluster", action="store_false", default=True)
     s.add_argument("--profile", default=None, choices=["coding", "multi-user"])
     s.add_argument("--max-model-len", type=int, default=None)
@@ -121,10 +125,16 @@ def build_parser() -> argparse.ArgumentParser:
     return p
 
 
+def _sparse(a) -> dict:
+    n = getattr(a, "sparse_pages", 0)
+    return {"sparse_pages": n} if n else {}
+
+
 def _cmd_run(a) -> int:
     from .pipeline import InferencePipeline
     pipe = InferencePipeline(verbose=True).load(a.model, num_gpus=a.gpus, quantization=resolve_quantization(a.quantization),
-                                                num_layers=a.num_layers)
+                                                num_layers=a.num_layers,
+                                                **_sparse(a))
     try:
         if a.prompt is not None:
             for delta in pipe.generate_stream(a.prompt, max_new_tokens=a.max_tokens, temperature=a.temperature):
@@ -167,6 +177,7 @@ def _cmd_serve(a) -> int:
         kw = {}
         if a.max_model_len:
             kw["max_model_len"] = a.max_model_len
+        kw.update(_sparse(a))
         pipe = InferencePipeline().load(model, num_gpus=a.gpus, quantization=resolve_quantization(a.quantization),
                                         num_layers=a.num_layers, **kw)
     if int(os.environ.get("RANK", "0")) != 0:

@@ -30,7 +30,8 @@ from ..models.transformer import DecoderModel, ForwardBatch
 from ..models.weights import random_weights
 
 DEFAULT_PORT = 18951
-_BATCH_TENSORS = [f.name for f in fields(ForwardBatch) if f.name not in ("is_decode", "max_q_len", "attn_splits")]
+_BATCH_TENSORS = [f.name for f in fields(ForwardBatch)
+                  if f.name not in ("is_decode", "max_q_len", "attn_splits", "decode_rows")]
 
 
 def _pack_batch(batch: ForwardBatch) -> Dict[str, torch.Tensor]:

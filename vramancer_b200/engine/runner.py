@@ -282,7 +282,10 @@ class ModelRunner:
             self.model.copy_pages(pairs)
             return
         for src, dst in pairs:
-            self.pool.cache[dst].copy_(self.pool.cache[src])
+            if hasattr(self.pool, "copy_page"):
+                self.pool.copy_page(src, dst)
+            else:
+                self.pool.cache[dst].copy_(self.pool.cache[src])
 
     def release_graphs(self) -> None:
         self._graphs.clear()
@@ -377,7 +380,7 @@ class ModelRunner:
         g = lambda k: views[k][0]   # noqa: E731
         batch = ForwardBatch(input_ids=g("ids"), positions=g("pos"), slot_mapping=g("slots"),
                              block_tables=g("bt").view(B, self.max_pages), context_lens=g("ctx"), is_decode=False,
-                             cu_q=g("cu"), max_q_len=T, logits_rows=None)
+                             cu_q=g("cu"), max_q_len=T, logits_rows=None, decode_rows=True)
         vp = self._vp_model
         if vp:
             self.model.set_vp_logits(True)
@@ -450,8 +453,10 @@ class ModelRunner:
         o = h_out.numpy()
         return [o[r * T:r * T + len(it.token_ids)].tolist() for r, it in enumerate(items)]
 
-    def prefill_logits(self, items: List[PrefillItem]) -> torch.Tensor:
-        """Prefill returning the raw logits rows (for scoring / speculative verify)."""
+    def prefill_logits(self, items: List[PrefillItem], decode_rows: bool = False) -> torch.Tensor:
+        """Prefill returning the raw logits rows (for scoring / speculative verify).
+        `decode_rows`: the tokens are fed for decoding (a verify step), so with
+        block-sparse decode they read selected pages as a decode step does."""
         dev = self.device
         ids, pos, slots, cu, ctx = [], [], [], [0], []
         maxp = max(len(it.block_table) for it in items)
@@ -468,5 +473,6 @@ class ModelRunner:
         i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)
         batch = ForwardBatch(input_ids=i32(ids), positions=i32(pos), slot_mapping=i32(slots),
                              block_tables=bt.to(dev), context_lens=i32(ctx), is_decode=False, cu_q=i32(cu),
-                             max_q_len=max(len(it.token_ids) for it in items), logits_rows=None)
+                             max_q_len=max(len(it.token_ids) for it in items), logits_rows=None,
+                             decode_rows=decode_rows)
         return self.model.forward(batch, self.pool)

@@ -192,7 +192,7 @@ def speculative_decode_step(engine, active, ngram: int, num_draft: int, stats: S
         vg = runner.verify_greedy(items)
         if vg is not None:
             return _accept_all_greedy(engine, active, feeds, starts, ds, [t for row in vg for t in row], stats)
-    logits = runner.prefill_logits(items)
+    logits = runner.prefill_logits(items, decode_rows=True)
     if logits.is_cuda:
         preds = ops.argmax(logits).cpu().tolist()
     else:

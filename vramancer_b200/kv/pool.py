@@ -12,6 +12,10 @@ pools store four-bit rows (`kv.q4`): the last dimension is the row's byte count,
 head_dim * 5 / 8, and a page takes 5/16 of the bf16 page's bytes.  int8 pools store
 TurboQuant records (`kv.turboquant`, 64 bytes per 128-dim row, 1/4 of bf16).
 
+With `key_bounds=True` a pool also holds, per page, layer and kv head, the elementwise
+minimum and maximum of the page's keys (`ops.key_bounds_for`; 1/16 of a bf16 or fp8
+pool's bytes), from which block-sparse decode chooses the pages it reads.
+
 Reference parity: the pool tensor of core/paged_attention.py:277-351 (same page
 shape and bytes/page, core/paged_attention.py:107-111).
 """
@@ -74,9 +78,12 @@ class KVPoolSpec:
 
 
 class KVPool:
-    """Owns the page tensor (and fp8 scales) on one device."""
+    """Owns the page tensor (and fp8 scales, key bounds) on one device."""
 
-    def __init__(self, spec: KVPoolSpec, device="cpu", kv_scale: Optional[torch.Tensor] = None):
+    key_bounds: Optional[torch.Tensor] = None
+
+    def __init__(self, spec: KVPoolSpec, device="cpu", kv_scale: Optional[torch.Tensor] = None,
+                 key_bounds: bool = False):
         self.spec = spec
         self.device = torch.device(device)
         shape = (spec.num_pages, spec.num_layers, 2, spec.kv_heads, spec.page_size, spec.row)
@@ -97,9 +104,21 @@ class KVPool:
         else:
             self.kv_scale = None
 
+        if key_bounds:
+            if self.is_tq:
+                raise ValueError("key bounds need bf16, fp8 or four-bit pages (not TurboQuant records)")
+            from .. import ops
+            self.key_bounds = ops.key_bounds_for(self.cache)
+
     @property
     def num_pages(self) -> int:
         return self.spec.num_pages
+
+    def copy_page(self, src: int, dst: int) -> None:
+        """Page src of every layer into page dst (copy-on-write), key bounds included."""
+        self.cache[dst].copy_(self.cache[src])
+        if self.key_bounds is not None:
+            self.key_bounds[dst].copy_(self.key_bounds[src])
 
     def page(self, idx: int) -> torch.Tensor:
         return self.cache[idx]
@@ -110,7 +129,9 @@ class KVPool:
             self.kv_scale.copy_(scale.to(self.kv_scale.device, torch.float32).view_as(self.kv_scale))
 
     def nbytes(self) -> int:
-        return self.cache.numel() * self.cache.element_size()
+        kb = self.key_bounds
+        return (self.cache.numel() * self.cache.element_size()
+                + (kb.numel() * kb.element_size() if kb is not None else 0))
 
 
 def calibrate_kv_scale(k_amax: torch.Tensor, v_amax: torch.Tensor, margin: float = 1.25) -> torch.Tensor:

@@ -13,6 +13,12 @@ from GPU d's memory (kv/overflow.py) and read in place by the attention kernels,
 sequence may grow past the local pool; the memory returns to the lender when its pages
 are freed or reclaimed.
 
+With `sparse_pages=N` decode is block-sparse: the pool keeps the elementwise minimum and
+maximum of every page's keys, and each decoded token reads at most N pages (16 tokens
+each) per layer and kv head: the first `sparse_sinks`, the last `sparse_recent`, and of
+the others those whose bounds allow the largest scores.  Contexts of up to N pages, and
+prompts, read everything.
+
 With `fold_norms=True` (the default; dense RMSNorm models with bf16 weights on one
 GPU) the input and post-attention RMSNorm weights are multiplied into the columns of
 `qkv_w` / `gate_up_w` in place, so small decode batches run the norms inside the
@@ -56,7 +62,8 @@ class LLM:
                  spec_num_draft: int = 0, spec_ngram: int = 3, kv_offload_pages: int = 0, hierarchy=None,
                  stream_layers: int = 0, ep=None, fold_norms: bool = True, pp_grid=None,
                  prefill_microbatches: int = 0, decode_microbatches: int = 1, kv_lender: Optional[int] = None,
-                 kv_borrow_pages: int = 0, lending_pool=None):
+                 kv_borrow_pages: int = 0, lending_pool=None, sparse_pages: int = 0, sparse_sinks: int = 1,
+                 sparse_recent: int = 2):
         if isinstance(model, ModelConfig):
             cfg = model
         else:
@@ -127,8 +134,15 @@ class LLM:
                 # small decode batches run the RMSNorms inside the GEMMs (weights folded in place)
                 self.model.fold_norms()
         kvd = kv_dtype_from_str(kv_cache_dtype)
+        if sparse_pages > 0:
+            if (kv_lender is not None or lending_pool is not None or kv_offload_pages > 0 or pp_grid is not None
+                    or kvd == torch.int8):
+                raise ValueError("sparse_pages needs a resident pool of bf16, fp8 or four-bit pages on one stage "
+                                 "(no kv_lender / lending_pool, kv_offload_pages, pp_grid or TurboQuant pages)")
+            self.model.set_sparse(sparse_pages, sparse_sinks, sparse_recent)
         if kv_pages is None:
-            kv_pages = self._pages_from_memory(cfg, kvd, gpu_memory_utilization, max_batch, max_model_len)
+            kv_pages = self._pages_from_memory(cfg, kvd, gpu_memory_utilization, max_batch, max_model_len,
+                                               key_bounds=sparse_pages > 0)
         spec = KVPoolSpec(kv_pages, self._kv_layers(), self.model.kvh, cfg.head_dim, dtype=kvd)
         if kv_lender is not None or lending_pool is not None:
             # VRAM lending: pages beyond the local pool are borrowed from another GPU's
@@ -137,7 +151,7 @@ class LLM:
             self.pool = ExtensiblePagePool(spec, self.device, kv_lender, kv_borrow_pages or kv_pages,
                                            lending_pool=lending_pool)
         else:
-            self.pool = KVPool(spec, self.device)
+            self.pool = KVPool(spec, self.device, key_bounds=sparse_pages > 0)
         self.offload = None
         if kv_offload_pages > 0 and enable_prefix_cache:
             # evicted prefix pages go to pinned host memory (and on to NVMe through `hierarchy`)
@@ -171,13 +185,15 @@ class LLM:
         """Layers whose KV this rank holds (a pipeline stage holds its own layers')."""
         return self.model.num_local_layers if self.pp_grid is not None else self.cfg.num_layers
 
-    def _pages_from_memory(self, cfg, kvd, util, max_batch, max_model_len) -> int:
+    def _pages_from_memory(self, cfg, kvd, util, max_batch, max_model_len, key_bounds: bool = False) -> int:
         need = max_batch * ((max_model_len + 15) // 16) + 16
         if self.device.type != "cuda":
             return min(need, 4096)
         free, total = torch.cuda.mem_get_info(self.device)
         budget = int(free - (1 - util) * total) - (2 << 30)   # keep ~2 GiB for activations/graphs
         per = KVPoolSpec(1, self._kv_layers(), self.model.kvh, cfg.head_dim, dtype=kvd).bytes_per_page
+        if key_bounds:
+            per += self._kv_layers() * self.model.kvh * 2 * cfg.head_dim * (1 if kvd == torch.float8_e4m3fn else 2)
         return max(16, min(need * 2, budget // per))
 
     # ------------------------------------------------------------------ API

@@ -47,6 +47,8 @@ class ForwardBatch:
     max_q_len: int = 1
     logits_rows: Optional[torch.Tensor] = None
     attn_splits: int = 0
+    # rows of a non-decode batch that are decoded, not prompt (a speculative verify step)
+    decode_rows: bool = False
 
     @property
     def num_tokens(self) -> int:
@@ -99,6 +101,7 @@ class DecoderModel:
         self.kvh = max(1, cfg.num_kv_heads // tps)
         self.D = cfg.head_dim
         self.sm_scale = 1.0 / math.sqrt(cfg.head_dim)
+        self.sparse = None           # (pages, sinks, recent) of block-sparse decode (set_sparse)
         self._rope_dummy = None      # one-page bf16 pool for RoPE without a KV write (TurboQuant pages)
         self.cos_sin = (ops.rope_cos_sin(cfg.max_position, cfg.rot_dim, cfg.rope_theta, self.device,
                                           scaling=cfg.rope_scaling)
@@ -197,6 +200,8 @@ class DecoderModel:
         cfg = self.cfg
         hq, kvh, D = self.hq, self.kvh, self.D
         qkv = self._in_proj(x, r, self.lw(i, "qkv_w"), self.lw(i, "qkv_b"))
+        if self.sparse is not None and pool.key_bounds is not None:
+            return self._attention_sparse(i, qkv, batch, pool)
         if cfg.qk_norm:          # Qwen3: per-head RMSNorm of q and k before RoPE
             ops.qk_rmsnorm(qkv, self.lw(i, "q_norm_w"), self.lw(i, "k_norm_w"), hq, kvh, D, cfg.norm_eps)
         li = i - self.first_layer
@@ -220,6 +225,39 @@ class DecoderModel:
         return ops.paged_attention_prefill(qkv, pool.cache, li, batch.block_tables, batch.cu_q,
                                            batch.context_lens, pool.kv_scale, self.sm_scale, hq,
                                            batch.max_q_len)
+
+    def set_sparse(self, pages: int, sinks: int = 1, recent: int = 2) -> None:
+        """Block-sparse decode: every decoded token reads at most `pages` pages per layer and
+        kv head, the first `sinks` and the last `recent` among them (`ops.select_pages`).
+        Prompts still read everything.  Needs a pool with key bounds."""
+        if sinks < 0 or recent < 1 or pages < sinks + recent:
+            raise ValueError("block-sparse decode needs sinks >= 0, recent >= 1 and pages >= sinks + recent")
+        if self.D not in (64, 128) or self.hq % self.kvh or self.hq // self.kvh > 8:
+            raise ValueError("block-sparse decode needs head_dim 64 or 128 and at most 8 query heads per kv head")
+        self.sparse = (pages, sinks, recent)
+
+    def _attention_sparse(self, i: int, qkv: torch.Tensor, batch: ForwardBatch, pool: KVPool) -> torch.Tensor:
+        """Attention over a pool with key bounds: one kernel normalises (Qwen3), rotates and
+        stores the new tokens and updates their pages' bounds; decoded rows then read their
+        selected pages, prompt rows all of them."""
+        cfg, hq, kvh = self.cfg, self.hq, self.kvh
+        li = i - self.first_layer
+        wq, wk = (self.lw(i, "q_norm_w"), self.lw(i, "k_norm_w")) if cfg.qk_norm else (None, None)
+        q = ops.qk_norm_rope_kv_write(qkv, wq, wk, cfg.norm_eps, batch.positions, self.cos_sin, pool.cache,
+                                      batch.slot_mapping, pool.kv_scale, li, hq, kvh, self.D,
+                                      key_bounds=pool.key_bounds)
+        bt, ctx = batch.block_tables, batch.context_lens
+        pages, sinks, recent = self.sparse
+        if bt.shape[1] <= pages or not (batch.is_decode or batch.decode_rows):    # every page is read
+            if batch.is_decode:
+                return ops.paged_attention_decode(q, pool.cache, li, bt, ctx, pool.kv_scale, self.sm_scale, hq,
+                                                  num_splits=batch.attn_splits)
+            return ops.paged_attention_prefill(q, pool.cache, li, bt, batch.cu_q, ctx, pool.kv_scale, self.sm_scale,
+                                               hq, batch.max_q_len)
+        cu_q = None if batch.is_decode else batch.cu_q
+        sel = ops.select_pages(q, pool.key_bounds, li, bt, ctx, hq, pages, sinks=sinks, recent=recent, cu_q=cu_q)
+        return ops.paged_attention_selected(q, pool.cache, li, bt, ctx, sel, pool.kv_scale, self.sm_scale, hq,
+                                            cu_q=cu_q)
 
     def _o_prefetch(self, i: int) -> Optional[torch.Tensor]:
         """The tensor holding layer i's o_proj weights (bf16 / fp8 matrix, or NVFP4

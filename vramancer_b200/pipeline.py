@@ -105,6 +105,8 @@ class InferencePipeline:
                 from .parallel.follower import StepBroadcaster
                 self._bcast = StepBroadcaster()
             elif has_cuda and num_gpus > 1:
+                if kw.get("sparse_pages"):
+                    raise ValueError("sparse_pages is not supported by the in-process layer pipeline (num_gpus > 1)")
                 self.llm = self._build_pp(cfg, num_gpus, max_batch, max_model_len, kv_pages, kvd, dtype, **kw)
                 self.mode = f"pp{num_gpus}"
             else:

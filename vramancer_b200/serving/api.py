@@ -492,7 +492,7 @@ def create_app(pipeline=None, *, model_alias: Optional[str] = None) -> FastAPI:
         if not name:
             return _err(400, "model required")
         kw = {k: body[k] for k in ("num_gpus", "max_batch", "max_model_len", "kv_cache_dtype", "num_layers",
-                                   "device") if k in body}
+                                   "device", "sparse_pages") if k in body}
         loop = asyncio.get_running_loop()
         try:
             await loop.run_in_executor(None, lambda: reg.load(name, **kw))

@@ -105,7 +105,7 @@ def _build(args, dev, tp, *, max_batch: int, max_len: int, kv_pages: Optional[in
         kw.setdefault("pp_grid", _PP_GRID)
     return LLM(args.model, device=str(dev), kv_cache_dtype=args.kv_dtype, max_batch=max_batch,
                max_model_len=max_len, kv_pages=kv_pages, quantization=args.quantization, tp=tp,
-               num_layers=args.num_layers, **kw)
+               num_layers=args.num_layers, sparse_pages=args.sparse_pages, **kw)
 
 
 def _pct(xs: List[float], q: float) -> float:
@@ -349,6 +349,7 @@ def parse_args(argv=None):
     ap.add_argument("--quantization", default=None, choices=[None, "nvfp4", "fp8"])
     ap.add_argument("--kv-dtype", default="bf16")
     ap.add_argument("--num-layers", type=int, default=None, help="debug only: truncated model")
+    ap.add_argument("--sparse-pages", type=int, default=0, help="block-sparse decode: pages a token reads (0: all)")
     ap.add_argument("--seed", type=int, default=0)
     ap.add_argument("--requests", type=int, default=64)
     ap.add_argument("--min-prompt", type=int, default=128)
