@@ -53,6 +53,15 @@ __device__ __forceinline__ uint32_t fp8x2_to_half2(uint32_t v) {
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)v));
   return r;
 }
+// the four e4m3 of v (exact)
+__device__ __forceinline__ void fp8x4_to_half4(uint32_t v, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 l, h;\n\t"
+      "mov.b32 {l, h}, %2;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %0, l;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(v));
+}
 __device__ __forceinline__ float ex2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -168,9 +177,10 @@ __device__ __forceinline__ void unpack8(uint4 v, float* x) {
 __device__ __forceinline__ uint4 pack8(const float* x) {
   return make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
 }
-// four e4m3 codes -> 2 x f16x2 (exact)
 __device__ __forceinline__ uint2 fp8x4_to_half4(uint32_t v) {
-  return make_uint2(fp8x2_to_half2(v), fp8x2_to_half2(v >> 16));
+  uint2 r;
+  fp8x4_to_half4(v, r.x, r.y);
+  return r;
 }
 
 // One rounding from fp32 to the page format.  dst: the stored row; `on`: this lane's row is
@@ -581,12 +591,13 @@ void qk_norm_rope_kv_write(const AppendArgs& in, cudaStream_t st) {
 // Which page is the last to be taken depends on differences of any size, so the choice is
 // the one that 64-bit sums make (products of 8-bit significands are exact there), ties to
 // the lowest page.  64-bit arithmetic for every page would cost more than reading it, so
-// pages are first scored in fp32 by the tensor cores: 16 pages are the rows of an MMA, their
-// bounds go from memory to its A operand as they are, and the query vector is split into
-// three 16-bit parts (24 bits of it) that fill three of the eight columns.  With S an upper
-// bound of sum |term|, such a score is off by less than E = 2^-18 S (an MMA from zero adds 16
-// exact products, each off by at most 2^-23 of their largest magnitude: 2^-19 S over all of
-// them, and the 18 fp32 additions of their sums 2^-19.8 S), so with the need-th largest score b every page above b + 2E is taken,
+// pages are first scored in fp32 by the tensor cores: bounds go from memory to the A operand
+// of an MMA as they are (e4m3 as f16), and the query vector is split into three 16-bit
+// parts (24 bits of it) that are columns of B.  With S an upper
+// bound of sum |term|, such a score is off by less than E = 2^-17 S (two MMAs in turn add 33
+// exact products and one sum, each off by at most 2^-23 of the sum of their magnitudes:
+// 2^-17.9 S over all of them, and the fp32 additions of their sums 2^-20 S), so with the
+// need-th largest score b every page above b + 2E is taken,
 // every page below b - 2E is not, and the few between are scored again in 64 bits.
 // Whatever fp32 cannot decide (S out of range, non-finite values, more pages between
 // than kSelList) is decided by 64-bit scores of all pages.
@@ -607,11 +618,6 @@ __device__ __forceinline__ void bf16x2_to_f64(uint32_t w, double& a, double& b) 
 __device__ __forceinline__ void fp8x4_to_f64(uint32_t w, double (&v)[4]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) v[i] = hi_word((uint32_t)((int32_t)(w << (24 - 8 * i)) >> 7) & 0x80FE0000u);
-}
-
-__device__ __forceinline__ uint32_t max_abs_half2(uint32_t a, uint32_t b) {
-  const __half2 r = __hmax2(__habs2(*reinterpret_cast<__half2*>(&a)), __habs2(*reinterpret_cast<__half2*>(&b)));
-  return *reinterpret_cast<const uint32_t*>(&r);
 }
 
 // unsigned keys in the order of the values
@@ -725,17 +731,25 @@ __device__ __forceinline__ void radix_pass(SelectScratch<NT>& sc, int n, F key, 
 }  // namespace
 
 // One cluster of 1, 2, 4 or 8 CTAs per (kv head, query row).  Every CTA scores a slice of
-// the row's candidate pages, 16 a warp at a time: lane (g, c) reads 16-byte pieces c, c + 4,
-// ... of pages g and g + 8, and each piece of the next 16 pages is requested as soon as the
-// MMAs have used the present one.  Scores go to the shared memory of the cluster's first
-// CTA, which chooses.
+// the row's candidate pages; scores go to the shared memory of the cluster's first CTA,
+// which chooses.
+//
+// Scoring is bound by the instructions a page takes as much as by memory, so the MMAs use the
+// bounds as loads deliver them: lane (g, c) reads 16-byte pieces c, c + 4, .. of page g, and
+// the four words of a piece are the lane's four A registers.  Words 0 and 2 thereby belong
+// to row g, words 1 and 3 to row g + 8: a page fills two rows, the query's parts for even
+// words are columns 0..2, for odd words columns 3..5, and a page's score is its first row's
+// columns 0..2 plus its second row's 3..5.  (e4m3 words become f16 pairs on the way.)  A warp
+// holds kTile pages in registers and requests the next ones' pieces as soon as the MMAs have
+// used the present ones'.
 template <int D, bool F8, int NT>
 __global__ void __launch_bounds__(NT, 512 / NT) select_kernel(SelectArgs a) {
   constexpr int kEl = F8 ? 1 : 2;
   constexpr int kPageB = 2 * D * kEl;            // bounds of one page and kv head
-  constexpr int kPieces = kPageB / 64;           // 16-byte pieces of a page per lane
-  constexpr int kSteps = 2 * D / 16;             // MMAs of 16 pages
-  constexpr int kSp = kSteps / kPieces;          // MMAs a piece feeds
+  constexpr int kPieces = kPageB / 64;           // 16-byte pieces of a page per lane: minima, then maxima
+  constexpr int kSp = F8 ? 2 : 1;                // MMAs a piece feeds
+  constexpr int kSteps = kPieces * kSp;          // MMAs of 8 pages
+  constexpr int kSub = kPieces == 8 ? 2 : 4, kTile = 8 * kSub;
   constexpr int kWarps = NT / 32;
   extern __shared__ __align__(16) uint8_t s_dyn[];
   float* s_score = reinterpret_cast<float*>(s_dyn);              // [max_pages] fp32 scores
@@ -769,8 +783,8 @@ __global__ void __launch_bounds__(NT, 512 / NT) select_kernel(SelectArgs a) {
   for (int i = tid; i < kBins / 4; i += NT) reinterpret_cast<uint4*>(sc.hist)[i] = make_uint4(0u, 0u, 0u, 0u);
   // and, where the warp's first pages do not depend on it, beside its block-table entries
   const bool early = nc == 1 && a.cu_q == nullptr;
-  const int first = a.sinks + warp * 16 + lane;
-  const int early_entry = early && lane < 16 && first < a.max_pages ? a.block_tables[(size_t)t * a.bt_stride + first] : 0;
+  const int first = a.sinks + warp * kTile + lane;
+  const int early_entry = early && lane < kTile && first < a.max_pages ? a.block_tables[(size_t)t * a.bt_stride + first] : 0;
   RowOf row;
   if (!find_row(t, a.cu_q, a.context_lens, a.B, row)) return;      // the same for the whole cluster
   int* out = a.out + ((size_t)t * a.KH + kvh) * a.budget;
@@ -796,36 +810,37 @@ __global__ void __launch_bounds__(NT, 512 / NT) select_kernel(SelectArgs a) {
   const uint8_t* bounds = reinterpret_cast<const uint8_t*>(a.bounds) + ((size_t)a.layer * a.KH + kvh) * kPageB;
   bool odd = false;                              // something that fp32 scores cannot decide
 
-  // lanes 0..15 hold the block-table entries of the warp's 16 pages
+  // lanes below kTile hold the block-table entries of the warp's pages
   auto entries = [&](int tile) -> int {
-    const int i = tile * 16 + lane;
-    return lane < 16 && i < m ? bt[c0 + i] : 0;
+    const int i = tile * kTile + lane;
+    return lane < kTile && i < m ? bt[c0 + i] : 0;
   };
-  const uint8_t *p0, *p1;                        // this lane's pieces of pages g, g + 8
   int* page0 = nullptr;
-  auto point = [&](int entry, int tile) {
+  auto check = [&](int entry, int tile) -> int {
     const bool bad = entry < 0 || entry >= a.num_pages;
     if (bad) report_error(a.err, kErrBounds);
     odd |= bad;
     entry = bad ? 0 : entry;
-    if (lane < 16 && tile * 16 + lane < m) page0[c0 + tile * 16 + lane] = entry;
-    p0 = bounds + (size_t)__shfl_sync(0xffffffffu, entry, g) * page_stride + c * 16;
-    p1 = bounds + (size_t)__shfl_sync(0xffffffffu, entry, g + 8) * page_stride + c * 16;
+    const int i = tile * kTile + lane;
+    if (lane < kTile && i < m) page0[c0 + i] = entry;
+    return entry;
   };
-  const int tiles = (m + 15) / 16;
-  uint32_t r[kPieces][2][4];
-  int entry0 = warp < tiles ? (early ? (warp * 16 + lane < m ? early_entry : 0) : entries(warp)) : 0;
+  const int tiles = (m + kTile - 1) / kTile;
+  uint32_t r[kSub][kPieces][4];
+  auto load = [&](int sub, int entry) {
+    const uint8_t* p = bounds + (size_t)__shfl_sync(0xffffffffu, entry, sub * 8 + g) * page_stride + c * 16;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) ld_stream<16>(r[sub][i], p + i * 64);
+  };
+  int entry = warp < tiles ? (early ? (warp * kTile + lane < m ? early_entry : 0) : entries(warp)) : 0;
   if (nc > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");   // the first CTA runs
   float* score0 = nc > 1 ? cluster.map_shared_rank(s_score, 0) : s_score;
   page0 = nc > 1 ? cluster.map_shared_rank(s_page, 0) : s_page;
   int next = 0;
   if (warp < tiles) {
-    point(entry0, warp);
+    entry = check(entry, warp);
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      ld_stream<16>(r[i][0], p0 + i * 64);
-      ld_stream<16>(r[i][1], p1 + i * 64);
-    }
+    for (int k = 0; k < kSub; ++k) load(k, entry);
     next = entries(warp + kWarps);
   }
   double qu = 0., qd = 0.;
@@ -880,74 +895,77 @@ __global__ void __launch_bounds__(NT, 512 / NT) select_kernel(SelectArgs a) {
     }
   }
   __syncthreads();
-  // B operand: column g < 3 is part g; step s takes four elements of the bounds' order
+  // B operand of step s: columns 0..2 and 3..5
   uint2 qb[kSteps];
 #pragma unroll
   for (int s = 0; s < kSteps; ++s) {
-    const int el = ((s / kSp) * 4 + c) * (16 / kEl) + (s % kSp) * 4;
-    qb[s] = g < 3 ? *reinterpret_cast<const uint2*>(&s_part[g < 3 ? g : 0][el]) : make_uint2(0u, 0u);
+    const int piece = ((s / kSp) * 4 + c) * (16 / kEl);            // its first element
+    const int el = F8 ? piece + (2 * (s % 2) + g / 3) * 4 : piece + (g / 3) * 2;
+    const uint16_t* p = &s_part[g % 3][g < 6 ? el : 0];
+    qb[s].x = g < 6 ? *reinterpret_cast<const uint32_t*>(p) : 0u;
+    qb[s].y = g < 6 ? *reinterpret_cast<const uint32_t*>(p + (F8 ? 2 : 4)) : 0u;
   }
 
   uint32_t key_hi = 0, key_lo_c = 0;             // largest key, largest complement
-  uint32_t amax = 0;                             // largest |bound| of the lane, both halves
+  // Largest maximum and most negative minimum of the lane's bounds, 16 bits each: a minimum
+  // is not above its maximum, so no bound is larger in magnitude than both.  As integers,
+  // positive values rise with their magnitude (signed order), negative ones too (unsigned).
+  uint32_t high = 0, deep = 0;
+  auto widest = [&](const uint32_t (&w)[4], bool is_max) {
+    if (is_max) high = __vimax3_s16x2(__vimax3_s16x2(high, w[0], w[1]), w[2], w[3]);
+    else deep = __vimax3_u16x2(__vimax3_u16x2(deep, w[0], w[1]), w[2], w[3]);
+  };
   for (int tile = warp; tile < tiles; tile += kWarps) {
     const bool more = tile + kWarps < tiles;
     if (more) {
-      point(next, tile + kWarps);
+      entry = check(next, tile + kWarps);
       next = entries(tile + 2 * kWarps);
     }
-    float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
+    for (int k = 0; k < kSub; ++k) {
+      // two MMAs a sum in the tensor core, the rest in fp32
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int w = 0; w < kSp; ++w) {
-        const int s = i * kSp + w;
+      for (int s2 = 0; s2 < kSteps; s2 += 2) {
         float acc[4] = {0.f, 0.f, 0.f, 0.f};
-        if constexpr (F8) {
-          const uint32_t a0 = fp8x2_to_half2(r[i][0][w]), a1 = fp8x2_to_half2(r[i][1][w]);
-          const uint32_t a2 = fp8x2_to_half2(r[i][0][w] >> 16), a3 = fp8x2_to_half2(r[i][1][w] >> 16);
-          mma_f16(acc, a0, a1, a2, a3, qb[s].x, qb[s].y);
-          amax = max_abs_half2(max_abs_half2(amax, a0), max_abs_half2(a1, max_abs_half2(a2, a3)));
-        } else {
-          mma_bf16_16816(acc, r[i][0][2 * w], r[i][1][2 * w], r[i][0][2 * w + 1], r[i][1][2 * w + 1], qb[s].x, qb[s].y);
+#pragma unroll
+        for (int s = s2; s < s2 + 2; ++s) {
+          uint32_t(&w)[4] = r[k][s / kSp];
+          const bool is_max = s >= kSteps / 2;
+          if constexpr (F8) {
+            uint32_t x[4];
+            fp8x4_to_half4(w[2 * (s % 2)], x[0], x[2]);
+            fp8x4_to_half4(w[2 * (s % 2) + 1], x[1], x[3]);
+            mma_f16(acc, x[0], x[1], x[2], x[3], qb[s].x, qb[s].y);
+            widest(x, is_max);
+          } else {
+            mma_bf16_16816(acc, w[0], w[1], w[2], w[3], qb[s].x, qb[s].y);
+            widest(w, is_max);
+          }
         }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) sum[k] += acc[k];
+        for (int x = 0; x < 4; ++x) sum[x] += acc[x];
       }
-      if constexpr (!F8) {
-#pragma unroll
-        for (int w = 0; w < 4; ++w)
-          amax = __vmaxu2(amax, __vmaxu2(r[i][0][w] & 0x7fff7fffu, r[i][1][w] & 0x7fff7fffu));
-      }
-      if (more) {
-        ld_stream<16>(r[i][0], p0 + i * 64);
-        ld_stream<16>(r[i][1], p1 + i * 64);
-      }
-    }
-    // columns 0, 1 lie in lanes c = 0, column 2 in c = 1
-    float v0 = sum[0] + sum[1], v1 = sum[2] + sum[3];
-    v0 += __shfl_xor_sync(0xffffffffu, v0, 1);
-    v1 += __shfl_xor_sync(0xffffffffu, v1, 1);
-    const int i0 = tile * 16 + g;
-    if (c == 0) {
-      odd |= (i0 < m && !isfinite(v0)) || (i0 + 8 < m && !isfinite(v1));
-      if (i0 < m) {
-        score0[c0 + i0] = v0;
-        key_hi = max(key_hi, sortable(v0));
-        key_lo_c = max(key_lo_c, ~sortable(v0));
-      }
-      if (i0 + 8 < m) {
-        score0[c0 + i0 + 8] = v1;
-        key_hi = max(key_hi, sortable(v1));
-        key_lo_c = max(key_lo_c, ~sortable(v1));
+      if (more) load(k, entry);
+      // this lane's columns 2c, 2c + 1: of row g 0..2 are wanted, of row g + 8 3..5
+      float v = c == 0 ? sum[0] + sum[1] : c == 1 ? sum[0] + sum[3] : c == 2 ? sum[2] + sum[3] : 0.f;
+      v += __shfl_xor_sync(0xffffffffu, v, 1);
+      v += __shfl_xor_sync(0xffffffffu, v, 2);
+      const int i = tile * kTile + k * 8 + g;
+      if (c == 0 && i < m) {
+        score0[c0 + i] = v;
+        odd |= !isfinite(v);
+        key_hi = max(key_hi, sortable(v));
+        key_lo_c = max(key_lo_c, ~sortable(v));
       }
     }
   }
   // infinite or NaN bounds (as bit patterns they are the largest), or fp32 cannot decide
-  uint32_t big = max(amax << 16, amax & 0xFFFF0000u);
+  const uint32_t wide = __vmaxu2(high & 0x7fff7fffu, deep & 0x7fff7fffu);
+  uint32_t big = max(wide << 16, wide & 0xFFFF0000u);
   if constexpr (F8) {
-    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&amax));
-    big = __float_as_uint(fmaxf(fabsf(v.x), fabsf(v.y)));
+    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&wide));
+    big = __float_as_uint(fmaxf(v.x, v.y));
   }
   if (__any_sync(0xffffffffu, odd)) big = 0x7F800000u;
   big = __reduce_max_sync(0xffffffffu, big);
@@ -1010,8 +1028,8 @@ __global__ void __launch_bounds__(NT, 512 / NT) select_kernel(SelectArgs a) {
     // The need-th largest score lies in [lo, hi]: the bin of a histogram over the range of
     // all scores, then over the edges of that bin, until few share one (scores above hi
     // count in the top bin, which that score is not in).  A bin's edges are off by less than
-    // 2^-10 of its width; 2 E = 2^-17 S.
-    const float E2 = S * 7.62939453125e-06f;
+    // 2^-10 of its width; 2 E = 2^-16 S.
+    const float E2 = S * 1.52587890625e-05f;
     float lo = from_sortable(key_lo), hi = from_sortable(key_hi);
     uint32_t in_bin = (uint32_t)n;
     while (in_bin > 8 && hi - lo > E2) {
@@ -1185,19 +1203,21 @@ void select_pages(const SelectArgs& in, cudaStream_t st) {
   VRM_REQUIRE(a.D == 64 || a.D == 128, "select_pages: head_dim must be 64 or 128");
   VRM_REQUIRE(a.max_pages <= kSelMaxPages, "select_pages: more than 24576 pages a sequence");
   VRM_REQUIRE(a.T <= 65535, "select_pages: too many query rows");
-  // Few rows: a cluster shares a row's candidates, as long as all CTAs fit two to an SM.
-  // Many: CTAs of 4 warps, four to an SM, so that one's choosing hides behind the others'
-  // reading.  B200, 32k tokens, D = 128, 8 kv heads (us): 1 row 22.9 / 16.4 / 13.0 / 11.7 with
-  // 1 / 2 / 4 / 8 CTAs, 16 rows 39.8 / 30.0 / 34.7 / 43.1; 8 against 4 warps: 32 rows of 16k
-  // tokens 27.0 / 38.7, 64 rows of fp8 bounds 64.5 / 58.1.
-  const long long rows = (long long)a.T * a.KH, fit = 2ll * device_sm_count();
+  // Few rows: CTAs of 16 warps, one to an SM, and a cluster shares a row's candidates as long
+  // as every CTA has its SM.  More: one CTA a row, of 8 warps while two to an SM hold all rows,
+  // else of 4, four to an SM.  B200, 8 kv heads of 128 dims (us): 1 row of 32k tokens with 1 / 2 / 4 / 8
+  // CTAs 19.1 / 14.2 / 11.3 / 9.9, 4 rows 21.4 / 15.7 / 12.6 / 20.1, 16 rows 25.5 / 31.1 / 41.2 /
+  // 54.2; 16, 8 and 4 warps a CTA: 16 rows 25.5, 27.1 (2 CTAs), 36.1; 32 rows of 16k 29.0,
+  // 24.8, 33.8; 64 rows of fp8 bounds at 32k -, 62.4, 58.1.
+  const long long rows = (long long)a.T * a.KH, sms = device_sm_count();
   int nc = 1;
-  while (nc < 8 && rows * nc * 2 <= fit) nc *= 2;
+  while (nc < 8 && rows * nc * 2 <= sms) nc *= 2;
   auto go = [&](auto d, auto f8) {
     constexpr int D = decltype(d)::value;
     constexpr bool F8 = decltype(f8)::value;
-    if (rows <= fit) launch_select<D, F8, 256>(a, nc, st);
-    else launch_select<D, F8, 128>(a, nc, st);
+    if (rows <= sms) launch_select<D, F8, 512>(a, nc, st);
+    else if (rows <= 2 * sms) launch_select<D, F8, 256>(a, 1, st);
+    else launch_select<D, F8, 128>(a, 1, st);
   };
   using D128 = std::integral_constant<int, 128>;
   using D64 = std::integral_constant<int, 64>;
