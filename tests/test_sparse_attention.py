@@ -248,6 +248,23 @@ def test_append_rewrites_and_reuses_pages(dev):
     assert put([4.0] * 15, 1) == (4, 5)
 
 
+@pytest.mark.parametrize("dev", DEVICES)
+def test_append_rising_slots_with_gaps(dev):
+    """Tokens of a page in rising slots that leave some out: the rows between count as they
+    are in the pool."""
+    Hq, KH, D = 2, 1, 64
+    cache = torch.zeros(2, 1, 2, KH, 16, D).bfloat16()
+    cache[1, 0, 0, 0, :, 0] = torch.arange(16).bfloat16() - 20
+    cache = cache.to(dev)
+    kb = ops.key_bounds_for(cache)
+    qkv = torch.zeros(4, (Hq + 2 * KH) * D)
+    qkv[:, Hq * D] = torch.tensor([1.0, 2.0, 3.0, -4.0])
+    ops.qk_norm_rope_kv_write(qkv.bfloat16().to(dev), None, None, 0.0, None, None, cache, i32([16, 19, 26, 1], dev),
+                              None, 0, Hq, KH, D, key_bounds=kb)
+    assert kb[1, 0, 0, :, 0].tolist() == [-19.0, 3.0]          # rows 1..9 but 3: -19 .. -11
+    assert kb[0, 0, 0, :, 0].tolist() == [-4.0, 0.0]
+
+
 # ---------------------------------------------------------------------------- selection
 def rows_of(T, ctx, cu):
     if cu is None:
@@ -351,6 +368,23 @@ def test_select_all_pages_alike(dev, same):
     bt = torch.arange(100, dtype=torch.int32)[None]
     got = ops.select_pages(torch.ones(1, 64).bfloat16().to(dev), kb.to(dev), 0, bt.to(dev), i32([1600], dev), 1, 20)
     assert got[0, 0].tolist() == list(range(19)) + [99]
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float8_e4m3fn])
+def test_select_many_equal_scores_at_the_border(dev, dt):
+    """Hundreds of pages tie around the border (more than a short list holds), others lie
+    above and below: the lowest of the tied."""
+    n = 1001
+    kb = torch.full((n, 1, 1, 2, 64), 1.0)
+    kb[::7] = 2.0
+    kb[3::7] = 0.5
+    bt = torch.arange(n, dtype=torch.int32)[None]
+    got = ops.select_pages(torch.ones(1, 64).bfloat16().to(dev), kb.to(dt).to(dev), 0, bt.to(dev),
+                           i32([16 * n], dev), 1, 400, sinks=0, recent=1)
+    v = kb[:n - 1, 0, 0, 1, 0].tolist()
+    want = sorted(range(n - 1), key=lambda p: (-v[p], p))[:399]
+    assert got[0, 0].tolist() == sorted(want) + [n - 1]
 
 
 @pytest.mark.parametrize("dev", DEVICES)

@@ -107,7 +107,7 @@ __device__ __forceinline__ bool find_row(int t, const int* cu_q, const int* cont
 // rotated pair sit in one lane; a 128-thread block takes kRows rows at a time.
 // A block takes a group of q heads or of v heads of a tile of kRows tokens, or one k head of
 // a k tile.  With key bounds a k block owns the runs (maximal sequences of adjacent tokens
-// in consecutive slots of one page) that begin in its tile, wherever they end, so every
+// in rising slots of one page) that begin in its tile, wherever they end, so every
 // page's bounds have one writer and do not depend on the order of the blocks.
 template <int D>
 struct AppendShape {
@@ -468,7 +468,7 @@ __global__ void __launch_bounds__(128) append_kernel(AppendArgs a) {
       bool st = true;
       if (i < in_tile + kPageTok - 1 && tile0 + i < a.T) {
         const int prev = s_slot[i], cur = s_slot[i + 1];
-        st = !(prev >= 0 && cur == prev + 1 && cur % kPageTok != 0);
+        st = !(prev >= 0 && cur > prev && cur / kPageTok == prev / kPageTok);
       }
       starts |= (uint64_t)__ballot_sync(0xffffffffu, st) << (32 * k);
     }
@@ -500,8 +500,8 @@ __global__ void __launch_bounds__(128) append_kernel(AppendArgs a) {
   }
   if (a.bounds == nullptr) return;
   __syncthreads();
-  // ---- bounds: one warp a run, D / 8 lanes a row.  The rows of the page before the run
-  // come from the pool (written by earlier calls), the run's own from shared memory.
+  // ---- bounds: one warp a run, D / 8 lanes a row, rows up to the run's last.  The run's own
+  // come from shared memory, the others from the pool (written by earlier calls).
   constexpr int kPer = D / 8, kGroups = 32 / kPer;
   const int lane = tid & 31, d8 = lane % kPer, grp = lane / kPer;
   for (int run = tid / 32; run < runs; run += 4) {
@@ -513,13 +513,16 @@ __global__ void __launch_bounds__(128) append_kernel(AppendArgs a) {
     uint4 lo = make_uint4(kInf, kInf, kInf, kInf), hi = lo;
     hi.x = hi.y = hi.z = hi.w = kInf | 0x80008000u;
     const uint8_t* base = kv_row(page, 0, 0, h);
-    const int old = slot % kPageTok;
+    const uint32_t rows = __reduce_or_sync(0xffffffffu, k0 + lane < k1 ? 1u << (s_slot[k0 + 1 + lane] % kPageTok) : 0u);
+    const uint32_t others = (0xffffffffu >> __clz(rows)) & ~rows;
+    if (others != 0) {
 #pragma unroll
-    for (int r = 0; r < kPageTok; r += kGroups) {
-      if (r + grp < old) {
-        const uint4 v = load_key8<D, FMT>(base + (r + grp) * kRowB, d8);
-        pick8<FMT, false>(lo, v);
-        pick8<FMT, true>(hi, v);
+      for (int r = 0; r < kPageTok; r += kGroups) {
+        if (others >> (r + grp) & 1u) {
+          const uint4 v = load_key8<D, FMT>(base + (r + grp) * kRowB, d8);
+          pick8<FMT, false>(lo, v);
+          pick8<FMT, true>(hi, v);
+        }
       }
     }
     for (int k = k0 + grp; k < k1; k += kGroups) {
@@ -1190,7 +1193,8 @@ template <int D, bool F8, int NT>
 static void launch_select(const SelectArgs& a, int nc, cudaStream_t st) {
   const size_t smem = (size_t)a.max_pages * sizeof(uint64_t);
   auto kern = select_kernel<D, F8, NT>;
-  if (smem > 32 * 1024) VRM_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  if (smem > 32 * 1024)
+    VRM_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelMaxPages * 8));
   const dim3 grid(nc, a.KH, a.T);
   if (nc > 1) launch_kernel_cluster(kern, grid, dim3(NT), dim3(nc, 1, 1), smem, st, a);
   else launch_kernel(kern, grid, dim3(NT), smem, st, a);

@@ -462,8 +462,8 @@ def qk_norm_rope_kv_write(qkv: torch.Tensor, wq: Optional[torch.Tensor], wk: Opt
     With `key_bounds` (`key_bounds_for`) every page that is written gets the elementwise
     minimum and maximum of its stored keys, from its first row to the last row written here
     (rows behind are not part of the sequence).  For that the tokens of a page must be
-    adjacent in the batch and in the order of their slots, as the tokens of a prefill chunk, a
-    verify step and a decode batch are.  Infinite keys count as the largest finite value of
+    adjacent in the batch, in rising slots, as the tokens of a prefill chunk, a verify step
+    and a decode batch are.  Infinite keys count as the largest finite value of
     the bounds' type, a NaN as both its extremes.  Slots must be distinct; a slot < 0 is not
     stored."""
     if qkv.is_cuda:
