@@ -2,6 +2,7 @@
 // launchers of vrm_kernels.h.  Every op runs on the current CUDA stream.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include "vrm_host.h"
@@ -394,6 +395,11 @@ void check_rows16(const Tensor& t, const char* name) {
               ": rows must start on 16-byte boundaries");
 }
 
+// A result of `ref`'s type and device (without the dispatcher: these calls are short)
+Tensor empty_beside(at::IntArrayRef size, const Tensor& ref) {
+  return at::detail::empty_cuda(size, ref.scalar_type(), ref.device(), c10::nullopt);
+}
+
 // key bounds [pages, layers, KH, 2, D]: bf16, or e4m3 (of fp8 pages)
 void check_bounds(const Tensor& b, const char* op) {
   TORCH_CHECK(b.is_cuda() && b.dim() == 5 && b.is_contiguous() && b.size(3) == 2 && b.numel() > 0, op,
@@ -460,7 +466,7 @@ Tensor qk_norm_rope_kv_write(const Tensor& qkv, const OptT& wq, const OptT& wk, 
     a.bounds = key_bounds->data_ptr();
   }
   const c10::cuda::CUDAGuard guard(qkv.device());
-  Tensor q = has(out) ? *out : torch::empty({T, Hq * D}, qkv.options());
+  Tensor q = has(out) ? *out : empty_beside({T, Hq * D}, qkv);
   check_rows16(q, "qk_norm_rope_kv_write out");
   TORCH_CHECK(q.size(0) >= T && q.size(1) >= Hq * D, op, ": out must be [T, Hq * D]");
   if (has(out) && q.is_alias_of(qkv)) {
@@ -533,7 +539,7 @@ Tensor select_pages(const Tensor& q, const Tensor& key_bounds, int64_t layer, co
   same_device(q, {&key_bounds}, op);
   same_device_opt(q, {&out}, op);
   const c10::cuda::CUDAGuard guard(q.device());
-  Tensor pages = has(out) ? *out : torch::empty({q.size(0), a.KH, budget}, block_tables.options());
+  Tensor pages = has(out) ? *out : empty_beside({q.size(0), a.KH, budget}, block_tables);
   TORCH_CHECK(pages.scalar_type() == torch::kInt32 && pages.is_contiguous() && pages.dim() == 3 &&
                   pages.size(0) >= q.size(0) && pages.size(1) == a.KH && pages.size(2) == budget,
               op, ": out must be contiguous int32 [T, kv_heads, budget]");
@@ -573,7 +579,7 @@ Tensor attn_selected(const Tensor& q, const Tensor& cache, int64_t layer, const 
     a.kv_scale = kv_scale->data_ptr<float>();
   }
   const c10::cuda::CUDAGuard guard(q.device());
-  Tensor o = has(out) ? *out : torch::empty({q.size(0), Hq * a.D}, q.options());
+  Tensor o = has(out) ? *out : empty_beside({q.size(0), Hq * a.D}, q);
   check_rows16(o, "paged_attention_selected out");
   TORCH_CHECK(o.size(0) >= q.size(0) && o.size(1) >= Hq * a.D, op, ": out must be [T, Hq * D]");
   a.cache = cache.data_ptr();
