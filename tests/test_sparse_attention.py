@@ -745,6 +745,8 @@ def test_refusals_cpu():
         with pytest.raises(ValueError):
             ops.select_pages(q, kb, 0, bt, ctx, 2, **bad)
     with pytest.raises(ValueError):
+        ops.select_pages(q, kb, 0, torch.zeros(1, ops.SELECT_MAX_PAGES + 1, dtype=torch.int32), ctx, 2, 3)
+    with pytest.raises(ValueError):
         ops.qk_norm_rope_kv_write(q, q[0, :64], None, 0.0, None, None, torch.zeros(1, 1, 2, 1, 16, 32).bfloat16(),
                                   ctx, None, 0, 2, 1, 32)
 
@@ -772,6 +774,7 @@ def test_refusals(cuda_errors_clean):
          dict(block_tables=bt.long()), dict(block_tables=bt[:1]), dict(context_lens=ctx[:1]),
          dict(context_lens=ctx.long()), dict(cu_q=torch.zeros(3, device=dev)), dict(cu_q=i32([0, 1, 2, 2], dev)),
          dict(key_bounds=kb.float()), dict(key_bounds=kb[:, :, :, :1]), dict(key_bounds=kb.cpu()),
+         dict(block_tables=torch.zeros(2, ops.SELECT_MAX_PAGES + 1, dtype=torch.int32, device=dev)),
          dict(out=pages.long()), dict(out=pages[:, :, :2]), dict(out=pages[:1])),
         (ops.paged_attention_selected, att, dict(layer=2), dict(num_q_heads=3), dict(num_q_heads=8),
          dict(q=q.half()), dict(cache=cache.float()), dict(cache=cache[:, :, :, :, :8]), dict(pages=pages.long()),

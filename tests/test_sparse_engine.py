@@ -125,6 +125,9 @@ def test_refusals():
         with pytest.raises(ValueError):
             cpu_llm(**kw)
     with pytest.raises(ValueError):
+        LLM("tiny-qwen3", device="cpu", dtype=torch.float32, kv_cache_dtype="fp32", max_batch=1, kv_pages=8,
+            max_model_len=16 * ops.SELECT_MAX_PAGES + 1, sparse_pages=4)
+    with pytest.raises(ValueError):
         KVPool(KVPoolSpec(2, 1, 1, 128, dtype=torch.int8), "cpu", key_bounds=True)
 
 

@@ -139,6 +139,9 @@ class LLM:
                     or kvd == torch.int8):
                 raise ValueError("sparse_pages needs a resident pool of bf16, fp8 or four-bit pages on one stage "
                                  "(no kv_lender / lending_pool, kv_offload_pages, pp_grid or TurboQuant pages)")
+            from . import ops
+            if (max_model_len + 15) // 16 > ops.SELECT_MAX_PAGES:
+                raise ValueError(f"sparse_pages serves contexts of up to {16 * ops.SELECT_MAX_PAGES} tokens")
             self.model.set_sparse(sparse_pages, sparse_sinks, sparse_recent)
         if kv_pages is None:
             kv_pages = self._pages_from_memory(cfg, kvd, gpu_memory_utilization, max_batch, max_model_len,

@@ -441,6 +441,9 @@ def paged_attention_prefill(q: torch.Tensor, cache: torch.Tensor, layer: int, bl
 
 
 # --------------------------------------------------------------------------- block-sparse decode
+SELECT_MAX_PAGES = 24576      # widest block table select_pages takes (393216 tokens)
+
+
 def key_bounds_for(cache: torch.Tensor) -> torch.Tensor:
     """Zeroed key bounds for a KV pool [pages, layers, 2, KH, 16, row]: [pages, layers, KH, 2, D]
     (minimum, maximum), bf16, or e4m3 codes (values before kv_scale) for fp8 pools."""
@@ -563,10 +566,14 @@ def select_pages(q: torch.Tensor, key_bounds: torch.Tensor, layer: int, block_ta
         sum_d ( sum_g max(q_gd, 0) * max_d  +  sum_g min(q_gd, 0) * min_d ),
 
     g over the query heads of the kv head: no key of the page gives the group a larger sum of
-    scores.  Scores are compared in 64 bits; ties go to the lowest page, a NaN comes first."""
+    scores (key_bounds hold min <= max, as the append leaves them).  Scores are compared in
+    64 bits; ties go to the lowest page, a NaN comes first.  Block tables have at most
+    SELECT_MAX_PAGES columns."""
     if q.is_cuda:
         return native().select_pages(q, key_bounds, layer, block_tables, context_lens, num_q_heads, budget, sinks,
                                      recent, cu_q, out)
+    if block_tables.shape[1] > SELECT_MAX_PAGES:
+        raise ValueError(f"select_pages: more than {SELECT_MAX_PAGES} pages a sequence")
     if sinks < 0 or recent < 1 or budget < sinks + recent:
         raise ValueError("select_pages: needs sinks >= 0, recent >= 1 and budget >= sinks + recent")
     T = q.shape[0]
@@ -604,8 +611,9 @@ def paged_attention_selected(q: torch.Tensor, cache: torch.Tensor, layer: int, b
                              out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of query rows (laid out as in `select_pages`) over the tokens of the listed
     pages only: pages int32 [T, KH, n] holds indexes into the row's block table, -1 (or any
-    page behind the row's context) for none.  Tokens behind the row's own are never read.  A
-    row without pages gives zeros; rows behind cu_q[B] are left as they were."""
+    page behind the row's context) for none; a page listed twice counts twice.  Tokens behind
+    the row's own are never read.  A row without pages gives zeros; rows behind cu_q[B] are
+    left as they were."""
     if q.is_cuda:
         return native().paged_attention_selected(q, cache, layer, block_tables, context_lens, pages, kv_scale,
                                                  sm_scale, num_q_heads, cu_q, out)
