@@ -916,7 +916,7 @@ __global__ void __launch_bounds__(NT, 512 / NT) select_kernel(SelectArgs a) {
     qb[s].y = g < 6 ? *reinterpret_cast<const uint32_t*>(p + (F8 ? 2 : 4)) : 0u;
   }
 
-  uint32_t key_hi = 0, key_lo_c = 0;             // largest key, largest complement
+  float s_hi = -INFINITY, s_lo = INFINITY;       // largest and smallest score of the lane, or NaN
   // Largest maximum and most negative minimum of the lane's bounds, 16 bits each: a minimum
   // is not above its maximum, so no bound is larger in magnitude than both.  As integers,
   // positive values rise with their magnitude (signed order), negative ones too (unsigned).
@@ -964,9 +964,8 @@ __global__ void __launch_bounds__(NT, 512 / NT) select_kernel(SelectArgs a) {
       const int i = tile * kTile + k * 8 + g;
       if (c == 0 && i < m) {
         score0[c0 + i] = v;
-        odd |= !isfinite(v);
-        key_hi = max(key_hi, sortable(v));
-        key_lo_c = max(key_lo_c, ~sortable(v));
+        asm("max.NaN.f32 %0, %0, %1;" : "+f"(s_hi) : "f"(v));
+        asm("min.NaN.f32 %0, %0, %1;" : "+f"(s_lo) : "f"(v));
       }
     }
   }
@@ -977,10 +976,11 @@ __global__ void __launch_bounds__(NT, 512 / NT) select_kernel(SelectArgs a) {
     const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&wide));
     big = __float_as_uint(fmaxf(v.x, v.y));
   }
+  odd |= !(s_hi < INFINITY && s_lo > -INFINITY);
   if (__any_sync(0xffffffffu, odd)) big = 0x7F800000u;
   big = __reduce_max_sync(0xffffffffu, big);
-  key_hi = __reduce_max_sync(0xffffffffu, key_hi);
-  key_lo_c = __reduce_max_sync(0xffffffffu, key_lo_c);
+  uint32_t key_hi = __reduce_max_sync(0xffffffffu, sortable(s_hi));
+  uint32_t key_lo_c = __reduce_max_sync(0xffffffffu, ~sortable(s_lo));     // largest complement
   if (lane < 3)
     (nc > 1 ? cluster.map_shared_rank(&s_ends[0][0], 0) : &s_ends[0][0])[(rank * kWarps + warp) * 3 + lane] =
         lane == 0 ? key_hi : lane == 1 ? key_lo_c : big;
