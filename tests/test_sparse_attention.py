@@ -694,6 +694,34 @@ def test_captured_and_replayed(cuda_errors_clean):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("width", [5000, ops.SELECT_MAX_PAGES])
+def test_captured_with_wide_tables(width, cuda_errors_clean):
+    """A table for very long contexts (more shared memory than a kernel has by default),
+    captured, replayed with other lengths, after a call with a narrow table."""
+    D, n = 64, 300
+    kb, _ = make_pool("bf16", n, 1, 1, D, "cuda")
+    kb = torch.stack([kb[:, :, 0, :, 0] - 1, kb[:, :, 0, :, 0] + 1], 3)
+    bt = torch.zeros(2, width, dtype=torch.int32, device="cuda")
+    bt[:, :n] = torch.arange(n, dtype=torch.int32, device="cuda")
+    q = torch.randn(2, D, generator=torch.Generator().manual_seed(0)).bfloat16().cuda()
+    ctx = i32([16 * n, 90], "cuda")
+    out = torch.empty(2, 1, 20, dtype=torch.int32, device="cuda")
+    call = lambda t: ops.select_pages(q, kb, 0, t, ctx, 1, 20, out=out)  # noqa: E731
+    call(bt)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        call(bt)
+    for lens in ([16 * n, 90], [1000, 16 * n - 7], [0, 400]):
+        ctx.copy_(i32(lens, "cuda"))
+        want = call(bt[:, :n].contiguous()).clone()
+        out.fill_(-5)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+
+
+@pytest.mark.gpu
 def test_other_streams_and_repeats(cuda_errors_clean):
     """Two streams at once, and the same call again: the same bits."""
     (s1, c1), (s2, c2) = gpu_step(seed=5), gpu_step(seed=6)
