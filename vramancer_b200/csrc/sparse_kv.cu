@@ -608,7 +608,7 @@ void qk_norm_rope_kv_write(const AppendArgs& in, cudaStream_t st) {
 // in 64 bits.  Whatever fp32 cannot decide (S out of range, non-finite values, more pages
 // between than kSelList) is decided by 64-bit scores of all pages.
 //
-// Bound by the reads while pages stream (64 rows of 32k tokens, fp8 bounds: 57.8 us, 4.7 TB/s;
+// Bound by the reads while pages stream (64 rows of 32k tokens, fp8 bounds: 56.4 us, 4.8 TB/s;
 // 23k tokens, bf16: 58.1 us, 5.1 TB/s), but a row's start and choice (about 15k cycles of
 // dependent loads, barriers and shared-memory passes) overlap other rows' reads only in part.
 namespace {
@@ -642,7 +642,10 @@ __device__ __forceinline__ uint32_t sortable(float s) {
 }
 __device__ __forceinline__ float from_sortable(uint32_t k) { return __uint_as_float(k >> 31 ? k & 0x7fffffffu : ~k); }
 
-constexpr int kSelList = 128;                    // pages decided by the short 64-bit path
+// Pages decided by the short 64-bit path.  An outlier channel makes E large beside the spread
+// of the scores: with 32 and one channel 400 times the others, 64 rows of 2048 pages of fp8
+// bounds took 471 us instead of 73, 1 row of 24576 pages 1105 instead of 43.
+constexpr int kSelList = 128;
 constexpr int kSelMaxPages = 24576;              // candidate pages of a row (8 bytes of shared memory each)
 constexpr int kBins = 1024;
 
@@ -1219,7 +1222,7 @@ void select_pages(const SelectArgs& in, cudaStream_t st) {
   // else of 4, four to an SM.  B200, 8 kv heads of 128 dims (us): 1 row of 32k tokens with 1 / 2 / 4 / 8
   // CTAs 19.1 / 14.2 / 11.3 / 9.9, 4 rows 21.4 / 15.7 / 12.6 / 20.1, 16 rows 25.5 / 31.1 / 41.2 /
   // 54.2; 16, 8 and 4 warps a CTA: 16 rows 25.5, 27.1 (2 CTAs), 36.1; 32 rows of 16k 29.0,
-  // 24.8, 33.8; 64 rows of fp8 bounds at 32k -, 62.4, 58.1.
+  // 24.8, 33.8; 64 rows of fp8 bounds at 32k -, 62.4, 56.4.
   const long long rows = (long long)a.T * a.KH, sms = device_sm_count();
   int nc = 1;
   while (nc < 8 && rows * nc * 2 <= sms) nc *= 2;
@@ -1398,7 +1401,9 @@ struct AttendShape {
 // warp requests its next page's K as soon as the scores have used the present one's, and V
 // after the outputs, so that loads are in flight all the time.  Splits are the CTAs of one
 // cluster: each pushes its partial outputs to the CTAs that finish them, through
-// distributed shared memory.
+// distributed shared memory.  Bound by the reads of the pages (32 rows of 128 bf16 pages:
+// 43.9 us, 6.1 TB/s; 128 rows of fp8: 92 us, 5.9 TB/s); one row is bound by the latency of
+// its table, pages and merge (7.7 us).
 template <int D, int FMT>
 __global__ void __launch_bounds__(128, AttendShape<D, FMT>::kCtas) attend_kernel(AttendArgs P) {
   using F = Frag<D, FMT>;
