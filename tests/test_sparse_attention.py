@@ -403,6 +403,33 @@ def test_select_close_scores(dev):
 
 @pytest.mark.parametrize("dev", DEVICES)
 @pytest.mark.parametrize("kind", ["bf16", "fp8"])
+@pytest.mark.parametrize("outlier", [8.0, 64.0, 416.0])
+@pytest.mark.parametrize("budget", [5, 128])
+def test_select_beside_an_outlier_channel(dev, kind, outlier, budget):
+    """One channel far above the others, alike in all pages: fp32 scores leave few to many
+    pages undecided.  All values are multiples of 1/16, so that 64-bit sums are exact."""
+    Hq, KH, D, ctx = 8, 2, 128, [16 * 1500, 16 * 300 - 3, 16 * 2000 + 1]
+    g = torch.Generator().manual_seed(int(outlier) + budget)
+    pages = sum(-(-n // 16) for n in ctx) + 1
+    bt = tables(ctx, 2001, pages, dev, 3)
+    step = 4 if kind == "fp8" else 16                         # e4m3 holds quarters up to 4
+    mid = torch.randint(-2 * step, 2 * step + 1, (pages, 1, KH, D), generator=g) / step
+    half = torch.randint(0, step + 1, (pages, 1, KH, D), generator=g) / step
+    kb = torch.stack([mid - half, mid + half], 3)
+    kb[..., 77] = outlier
+    dt = torch.float8_e4m3fn if kind == "fp8" else torch.bfloat16
+    assert torch.equal(kb.to(dt).float(), kb)
+    q = torch.randint(-32, 33, (3, Hq, D), generator=g) / 16
+    q[:, :, 77] = 4.0
+    kb, q = kb.to(dt).to(dev), q.bfloat16().view(3, Hq * D).to(dev)
+    got = ops.select_pages(q, kb, 0, bt, i32(ctx, dev), Hq, budget, sinks=1, recent=2).cpu()
+    want = select_ref(q, kb, 0, bt, rows_of(3, ctx, None), Hq, budget, 1, 2)
+    for (t, h), w in want.items():
+        assert got[t, h].tolist() == w, (t, h)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("kind", ["bf16", "fp8"])
 def test_select_extreme_values(dev, kind):
     """Largest and smallest finite values, subnormals, infinite and NaN queries."""
     dt = torch.bfloat16 if kind == "bf16" else torch.float8_e4m3fn
