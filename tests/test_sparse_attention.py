@@ -617,6 +617,71 @@ def test_attend_non_finite_scores(dev):
     assert (run(slice(0, 8), -math.inf) == 1.0).all()
 
 
+def small_pool(kind, dev, KH=1, D=64, pages=6, scale=1.0, seed=0):
+    cache, ks = make_pool(kind, pages, 1, KH, D, dev, seed, scale=scale)
+    return cache, ks, torch.arange(pages, dtype=torch.int32, device=dev)[None]
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("kind", ["bf16", "fp8", "q4"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("n_sel", [1, 40])
+def test_attend_heads_of_unlike_magnitudes(dev, kind, D, n_sel):
+    """Heads of one group whose queries lie 2^13 to 2^100 apart: each has its own scores."""
+    mags = [1.0, 2.0 ** 13, 2.0 ** 26, 2.0 ** 100, 0.0, 2.0 ** -30, 1.0]
+    cache, ks, bt = small_pool(kind, dev, D=D, pages=40, seed=D)
+    q = torch.randn(1, 7, D, generator=torch.Generator().manual_seed(D)) * torch.tensor(mags)[:, None]
+    q = q.bfloat16().view(1, 7 * D).to(dev)
+    pages = torch.arange(n_sel, dtype=torch.int32)[None, None]
+    got = ops.paged_attention_selected(q, cache, 0, bt, i32([640], dev), pages.to(dev), ks, 0.2, 7).cpu().double()
+    (o, tol), = attend_ref(q, values(cache, ks), 0, bt, {0: (0, 640)}, pages, 0.2, 7, kind).values()
+    e = (got.view(7, D) - o).abs()
+    assert torch.isfinite(got).all()
+    assert (e <= tol * (1 + 2.0 ** -10)).all(), (e - tol).amax(1)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("kind", ["bf16", "fp8", "q4"])
+@pytest.mark.parametrize("mag", [2.0 ** 124, 2.0 ** 125, 2.0 ** 126, 2.0 ** 127, 2.0 ** -120])
+def test_attend_largest_and_smallest_queries(dev, kind, mag):
+    """Finite queries of the last exponents are neither clipped nor taken for infinite.
+    Keys of at most 1/16 keep the products finite in 32 bits, and sm_scale is an fp32 value."""
+    cache, ks, bt = small_pool(kind, dev, scale=2.0 ** -7)
+    if kind == "fp8":
+        ks *= 2.0 ** -7
+        cache, _, _ = small_pool(kind, dev, scale=1.0)
+    assert values(cache, ks).abs().max() <= 1 / 16
+    q = torch.zeros(1, 2, 64)
+    q[0, 0, 5], q[0, 1, 9] = mag, -1.5 * mag
+    q = q.bfloat16().view(1, 128).to(dev)
+    pages = torch.arange(6, dtype=torch.int32)[None, None]
+    sm = 2.0 ** 7 / mag
+    got = ops.paged_attention_selected(q, cache, 0, bt, i32([90], dev), pages.to(dev), ks, sm, 2).cpu().double()
+    (o, tol), = attend_ref(q, values(cache, ks), 0, bt, {0: (0, 90)}, pages, sm, 2, kind).values()
+    e = (got.view(2, 64) - o).abs()
+    assert (e <= tol * (1 + 2.0 ** -10)).all(), (e - tol).amax(1)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("kind", ["bf16", "fp8", "q4"])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("n_sel", [1, 40])
+def test_attend_non_finite_queries(dev, kind, bad, n_sel):
+    """An infinite or NaN query value makes its own head NaN and no other."""
+    cache, ks, bt = small_pool(kind, dev, KH=2, pages=40)
+    q = torch.randn(1, 6, 64, generator=torch.Generator().manual_seed(7))
+    q[0, 1, 33] = bad
+    q = q.bfloat16().view(1, 6 * 64).to(dev)
+    pages = torch.arange(n_sel, dtype=torch.int32).repeat(1, 2, 1)
+    got = ops.paged_attention_selected(q, cache, 0, bt, i32([640], dev), pages.to(dev), ks, 0.125, 6).cpu().double()
+    got = got.view(6, 64)
+    assert got[1].isnan().all()
+    for (t, h), (o, tol) in attend_ref(q, values(cache, ks), 0, bt, {0: (0, 640)}, pages, 0.125, 6, kind).items():
+        for i in range(3):
+            if 3 * h + i != 1:
+                assert ((got[3 * h + i] - o[i]).abs() <= tol[i] * (1 + 2.0 ** -10)).all(), (h, i)
+
+
 # ---------------------------------------------------------------------------- as they are used
 @pytest.mark.parametrize("dev", DEVICES)
 @pytest.mark.parametrize("kind", ["bf16", "fp8", "q4"])

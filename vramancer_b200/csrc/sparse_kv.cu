@@ -1245,7 +1245,7 @@ namespace {
 
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   uint32_t r;
-  asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
@@ -1436,11 +1436,14 @@ __global__ void __launch_bounds__(128, AttendShape<D, FMT>::kCtas) attend_kernel
     for (int s = 0; s < kSteps; ++s)
       qb[s] = g < G ? *reinterpret_cast<const uint2*>(q + F::k_dim(s, c)) : make_uint2(0u, 0u);
   }
-  float scale_log2 = P.sm_scale * 1.4426950408889634f, v_scale = 1.f;
+  // factors of the scores of heads 2c and 2c + 1
+  float k_scale = 1.f, v_scale = 1.f;
   if constexpr (FMT == kFmtFp8) {
-    scale_log2 *= P.kv_scale[(P.layer * 2 + 0) * KH + kvh];
+    k_scale = P.kv_scale[(P.layer * 2 + 0) * KH + kvh];
     v_scale = P.kv_scale[(P.layer * 2 + 1) * KH + kvh];
   }
+  const float sm_log2 = P.sm_scale * 1.4426950408889634f;
+  float scale_log2[2] = {sm_log2 * k_scale, sm_log2 * k_scale};
   RowOf row;
   if (!find_row(t, P.cu_q, P.context_lens, P.B, row)) return;      // the same for the whole cluster
   if (nsplit > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // this CTA runs
@@ -1487,19 +1490,22 @@ __global__ void __launch_bounds__(128, AttendShape<D, FMT>::kCtas) attend_kernel
 #pragma unroll
     for (int q = 0; q < kTurn; ++q) f[q].load_v(kp[q] + (size_t)KH * head_b, r[q], g, c);
     if (!q_ready) {
-      // f16 operands: q times the power of two that brings its largest value to [1, 2)
+      // f16 operands: each head's q times the power of two that brings its largest value to
+      // [2^14, 2^15), or 2^126 if that is less: the eight bits of a value stay whole down to
+      // 2^-31 of the head's largest.  A head with an infinite value has no finite score: NaN.
       float mx = 0.f;
 #pragma unroll
       for (int s = 0; s < kSteps; ++s)
         mx = fmaxf(mx, fmaxf(fmaxf(fabsf(bf16_lo(qb[s].x)), fabsf(bf16_hi(qb[s].x))),
                              fmaxf(fabsf(bf16_lo(qb[s].y)), fabsf(bf16_hi(qb[s].y)))));
-      mx = warp_max(mx);
-      const int e = (int)(__float_as_uint(mx) >> 23);
-      float x = 1.f;
-      if (e > 1 && e < 253) {
-        x = __uint_as_float((uint32_t)(254 - e) << 23);
-        scale_log2 *= __uint_as_float((uint32_t)e << 23);
-      }
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      const uint32_t e = __float_as_uint(mx) >> 23, up = min(253u, 268u - e);
+      const float x = __uint_as_float(up << 23);
+      const float down = e == 255u ? NAN : __uint_as_float((254u - up) << 23);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        scale_log2[h] = sm_log2 * __shfl_sync(0xffffffffu, down, 4 * (2 * c + h)) * k_scale;
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
         qb[s].x = pack_half2(bf16_lo(qb[s].x) * x, bf16_hi(qb[s].x) * x);
@@ -1536,7 +1542,7 @@ __global__ void __launch_bounds__(128, AttendShape<D, FMT>::kCtas) attend_kernel
         if (more) f[q].load_k(kp[q], r[q], g, c);
         // sc[0] = (token g, head 2c), [1] = (g, 2c + 1), [2] = (g + 8, 2c), [3] = (g + 8, 2c + 1)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[q][i] = (sc[i] + sd[i]) * scale_log2;
+        for (int i = 0; i < 4; ++i) x[q][i] = (sc[i] + sd[i]) * scale_log2[i % 2];
         if (r_now[q] != kPageTok) {
           if (g >= r_now[q]) x[q][0] = x[q][1] = -INFINITY;
           if (g + 8 >= r_now[q]) x[q][2] = x[q][3] = -INFINITY;
