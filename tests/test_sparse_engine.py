@@ -131,6 +131,25 @@ def test_refusals():
         KVPool(KVPoolSpec(2, 1, 1, 128, dtype=torch.int8), "cpu", key_bounds=True)
 
 
+@pytest.mark.parametrize("n", [-1, -128])
+def test_negative_budget_is_refused(n, monkeypatch):
+    """Not taken for "off": by the engine, and by the commands and the model-load route that
+    pass it on."""
+    from fastapi.testclient import TestClient
+
+    from vramancer_b200 import cli
+    from vramancer_b200.serving.api import create_app
+    with pytest.raises(ValueError, match="negative"):
+        cpu_llm(sparse_pages=n)
+    for command in ("run", "serve"):
+        with pytest.raises(ValueError, match="negative"):
+            cli.main([command, "tiny-qwen2", "--sparse-pages", str(n)])
+    monkeypatch.setenv("VRM_API_TOKEN", "t")
+    r = TestClient(create_app()).post("/api/models/load", headers={"Authorization": "Bearer t"},
+                                      json={"model": "tiny-qwen2", "device": "cpu", "sparse_pages": n})
+    assert r.status_code == 500 and "negative" in r.text
+
+
 def test_command_line():
     from vramancer_b200.cli import build_parser
     a = build_parser().parse_args(["run", "m", "--sparse-pages", "64"])

@@ -134,6 +134,8 @@ class LLM:
                 # small decode batches run the RMSNorms inside the GEMMs (weights folded in place)
                 self.model.fold_norms()
         kvd = kv_dtype_from_str(kv_cache_dtype)
+        if sparse_pages < 0:
+            raise ValueError("sparse_pages must not be negative (0: read all pages)")
         if sparse_pages > 0:
             if (kv_lender is not None or lending_pool is not None or kv_offload_pages > 0 or pp_grid is not None
                     or kvd == torch.int8):
