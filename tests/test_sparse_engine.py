@@ -157,6 +157,24 @@ def test_command_line():
     assert build_parser().parse_args(["serve", "m"]).sparse_pages == 0
 
 
+def test_tensor_parallel_serve_relaunches_with_every_option(monkeypatch):
+    """`serve --tp N` starts itself once per GPU: the ranks parse the options that were given."""
+    from vramancer_b200 import cli
+    given = ["serve", "--model", "tiny-qwen2", "--tp", "2", "--sparse-pages", "64", "--max-model-len", "512",
+             "--quantization", "fp8", "--no-cluster", "--profile", "coding", "--num-layers", "1", "--host", "::1",
+             "--port", "5031"]
+    calls = []
+    monkeypatch.delenv("WORLD_SIZE", raising=False)
+    monkeypatch.setenv("VRM_N_CTX", "16384")                 # what --profile coding sets
+    monkeypatch.setattr(cli.subprocess, "call", lambda cmd: calls.append(cmd) or 0)
+    assert cli.main(given) == 0
+    cmd, = calls
+    at = cmd.index("vramancer_b200")
+    assert "--nproc-per-node=2" in cmd[:at]
+    parser = cli.build_parser()
+    assert vars(parser.parse_args(cmd[at + 1:])) == vars(parser.parse_args(given))
+
+
 # ------------------------------------------------------------------------- GPU
 def gpu_llm(model, kv, graph, **kw):
     return LLM(model, device="cuda", kv_cache_dtype=kv, max_batch=4, max_model_len=512, kv_pages=128,

@@ -165,10 +165,9 @@ def _cmd_serve(a) -> int:
     elif a.profile == "multi-user":
         os.environ.setdefault("VRM_MAX_BATCH_SIZE", "128")
     if a.tp > 1 and int(os.environ.get("WORLD_SIZE", "1")) == 1:
-        # relaunch one process per GPU; rank 0 serves HTTP, the others follow
+        # relaunch this command, one process per GPU; rank 0 serves HTTP, the others follow
         cmd = [sys.executable, "-m", "torch.distributed.run", "--nnodes=1", f"--nproc-per-node={a.tp}",
-               "--master-addr=127.0.0.1", "-m", "vramancer_b200", "serve", model, "--host", a.host, "--port",
-               str(a.port), "--tp", str(a.tp)]
+               "--master-addr=127.0.0.1", "-m", "vramancer_b200"] + a.argv
         return subprocess.call(cmd)
     from .serving.api import run_server
     from .pipeline import InferencePipeline
@@ -237,6 +236,7 @@ def _cmd_hub(a) -> int:
 def main(argv: Optional[List[str]] = None) -> int:
     p = build_parser()
     a = p.parse_args(argv)
+    a.argv = list(sys.argv[1:] if argv is None else argv)
     cmd = a.command
     if cmd is None:
         p.print_help()
