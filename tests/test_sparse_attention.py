@@ -456,6 +456,41 @@ def test_select_extreme_values(dev, kind):
     assert got[3, 0].tolist() == list(range(15)) + [39]
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["bf16", "fp8"])
+@pytest.mark.parametrize("rows,n", [(1, 6001), (3, 2999), (40, 1201)])
+def test_select_does_not_depend_on_other_sequences_pages(kind, rows, n, cuda_errors_clean):
+    """Pages that are not in a row's table cost it nothing, whatever keys they hold: page 0,
+    another sequence's, with the largest bounds.  A row that takes bf16 ones into its error
+    bound scores every page in 64 bits, 5 to 15 times as slow at these lengths."""
+    dt = torch.float8_e4m3fn if kind == "fp8" else torch.bfloat16
+    g = torch.Generator().manual_seed(n)
+    mid, half = torch.randn(n + 1, 1, 8, 128, generator=g), torch.rand(n + 1, 1, 8, 128, generator=g)
+    kb = torch.stack([mid - half, mid + half], 3).to(dt)
+    kb[0] = 0.0
+    loud = kb.clone()
+    loud[0, :, :, 0], loud[0, :, :, 1] = -torch.finfo(dt).max, torch.finfo(dt).max
+    bt = torch.stack([torch.randperm(n, generator=g).int() + 1 for _ in range(rows)]).cuda()
+    q = torch.randn(rows, 8 * 128, generator=g).bfloat16().cuda()
+    ctx = i32([16 * n - 3 * i for i in range(rows)], "cuda")
+    res, us = [], []
+    for b in (kb.cuda(), loud.cuda()):
+        call = lambda: ops.select_pages(q, b, 0, bt, ctx, 8, 128)  # noqa: E731,B023
+        res.append(call())
+        times = []
+        for _ in range(9):
+            a, z = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            for _ in range(5):
+                call()
+            z.record()
+            z.synchronize()
+            times.append(a.elapsed_time(z) * 200)
+        us.append(sorted(times)[4])
+    assert torch.equal(*res)
+    assert us[1] < 2 * us[0], us
+
+
 # ---------------------------------------------------------------------------- attention
 def attend_ref(q, vals, layer, bt, rows, pages, sm_scale, Hq, kind):
     """{(row, kv head): (output, tolerance)} in 64 bits."""

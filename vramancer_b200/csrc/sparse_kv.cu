@@ -823,11 +823,9 @@ __global__ void __launch_bounds__(NT, 512 / NT) select_kernel(SelectArgs a) {
   const uint8_t* bounds = reinterpret_cast<const uint8_t*>(a.bounds) + ((size_t)a.layer * a.KH + kvh) * kPageB;
   bool odd = false;                              // something that fp32 scores cannot decide
 
-  // lanes below kTile hold the block-table entries of the warp's pages
-  auto entries = [&](int tile) -> int {
-    const int i = tile * kTile + lane;
-    return lane < kTile && i < m ? bt[c0 + i] : 0;
-  };
+  // lanes below kTile hold the block-table entries of the warp's pages; behind the slice's
+  // last page it is repeated: a page that is not the row's would widen its S.  m > 0
+  auto entries = [&](int tile) -> int { return bt[c0 + min(tile * kTile + lane, m - 1)]; };
   int* page0 = nullptr;
   auto check = [&](int entry, int tile) -> int {
     const bool bad = entry < 0 || entry >= a.num_pages;
@@ -845,7 +843,8 @@ __global__ void __launch_bounds__(NT, 512 / NT) select_kernel(SelectArgs a) {
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) ld_stream<16>(r[sub][i], p + i * 64);
   };
-  int entry = warp < tiles ? (early ? (warp * kTile + lane < m ? early_entry : 0) : entries(warp)) : 0;
+  int entry = 0;
+  if (warp < tiles) entry = early ? __shfl_sync(0xffffffffu, early_entry, min(lane, m - 1 - warp * kTile)) : entries(warp);
   if (nc > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");   // the first CTA runs
   float* score0 = nc > 1 ? cluster.map_shared_rank(s_score, 0) : s_score;
   page0 = nc > 1 ? cluster.map_shared_rank(s_page, 0) : s_page;
