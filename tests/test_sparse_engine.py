@@ -26,6 +26,54 @@ def test_all_pages_is_dense(model):
     assert tokens(cpu_llm(model, sparse_pages=16)) == dense
 
 
+def count_selections(monkeypatch):
+    """A list that grows by one with every call of ops.select_pages."""
+    calls, real = [], ops.select_pages
+    monkeypatch.setattr(ops, "select_pages", lambda *a, **k: calls.append(1) or real(*a, **k))
+    return calls
+
+
+@pytest.mark.parametrize("model", ["tiny-qwen3", "tiny-qwen2", "tiny-gpt2", "tiny-moe"])
+def test_selection_of_all_pages_is_dense(model, monkeypatch):
+    """The block table is wider than the budget, the contexts are not: the selection lists
+    every page, and the tokens are the dense engine's."""
+    wide = dict(device="cpu", dtype=torch.float32, kv_cache_dtype="fp32", max_batch=4, max_model_len=512, kv_pages=96)
+    dense = tokens(LLM(model, **wide))
+    calls = count_selections(monkeypatch)
+    assert tokens(LLM(model, sparse_pages=16, **wide)) == dense
+    assert len(calls) >= 20
+
+
+def test_tensor_parallel():
+    """Two ranks, each with its own kv heads' bounds and selections: the tokens of one rank."""
+    from vramancer_b200.parallel.tensor_parallel import apply_tensor_parallel
+    kw = dict(max_batch=4, max_model_len=256, kv_pages=96)
+    one = tokens(cpu_llm("tiny-qwen3", sparse_pages=4), 12)
+    assert one != tokens(cpu_llm("tiny-qwen3"), 12)
+    tp = apply_tensor_parallel("tiny-qwen3", num_gpus=2, device="cpu", timeout_s=300, sparse_pages=4, **kw)
+    try:
+        assert tp.generate(PROMPTS, max_tokens=12) == one
+    finally:
+        tp.shutdown()
+
+
+def test_model_load_route(monkeypatch):
+    """`sparse_pages` of the load request reaches the engine that serves the model."""
+    from fastapi.testclient import TestClient
+
+    from vramancer_b200.serving.api import create_app
+    monkeypatch.setenv("VRM_API_TOKEN", "t")
+    calls = count_selections(monkeypatch)
+    with TestClient(create_app()) as c:
+        c.headers.update({"Authorization": "Bearer t"})
+        for budget in (0, 4):
+            r = c.post("/api/models/load", json={"model": "tiny-qwen2", "device": "cpu", "max_model_len": 256,
+                                                 "sparse_pages": budget})
+            assert r.status_code == 200, r.text
+            r = c.post("/v1/completions", json={"prompt": "x" * 120, "max_tokens": 3})
+            assert r.status_code == 200 and bool(calls) == (budget > 0), r.text
+
+
 def reference_step(llm, seq, budget, sinks, recent):
     """Greedy next token of `seq` with every token of it decoded block-sparse: a plain
     forward, one token after the other, over keys and values kept as tensors."""
@@ -229,3 +277,80 @@ def test_gpu_speculative_verify_graph(cuda_errors_clean):
     first = tokens(llm, 32, PROMPTS[:2])
     assert all(len(x) == 32 for x in first) and llm.runner._verify
     assert tokens(llm, 32, PROMPTS[:2]) == first
+
+
+def verify_step(llm, ids, bt, n):
+    """Logits of `ids`, the last of n tokens of a sequence in the pages `bt`, fed as a verify
+    step's rows."""
+    from vramancer_b200.models.transformer import ForwardBatch
+    m = len(ids)
+    t = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    pos = list(range(n - m, n))
+    return llm.model.forward(ForwardBatch(t(ids), t(pos), t([16 * bt[p // 16] + p % 16 for p in pos]), t([bt]), t([n]),
+                                          False, cu_q=t([0, m]), max_q_len=m, decode_rows=True), llm.pool)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("model,kv", [("tiny-qwen3", "bf16"), ("tiny-qwen2-d128", "bf16"), ("tiny-qwen2-d128", "fp8"),
+                                      ("tiny-qwen2-d128", "q4")])
+def test_gpu_selection_of_all_pages_is_dense(model, kv, cuda_errors_clean, monkeypatch):
+    """A step over a table wider than the budget: with every page selected the logits are
+    those of dense attention on the same pool, with four pages they are others."""
+    from vramancer_b200.engine.runner import PrefillItem
+    llm = gpu_llm(model, kv, False, sparse_pages=32, enable_prefix_cache=False)
+    ids = PROMPTS[0]
+    bt = list(range(3, 40))
+    slots = [16 * bt[p // 16] + p % 16 for p in range(len(ids))]
+    llm.runner.prefill([PrefillItem(ids, 0, slots, bt, len(ids), True)], [0.0], [0], [1.0], [0])
+    logits, calls = {}, count_selections(monkeypatch)
+    for name, sparse in (("dense", None), ("all", (32, 1, 2)), ("some", (4, 1, 2))):
+        llm.model.sparse = sparse
+        logits[name] = verify_step(llm, [9, 4, 7], bt, len(ids) + 3).float()
+        assert bool(calls) == (sparse is not None)
+    # bf16 activations through two layers: a few units of 2^-8 of the logits' scale
+    tol = 8 * 2.0 ** -8 * logits["dense"].abs().max()
+    assert (logits["all"] - logits["dense"]).abs().max() <= tol
+    assert (logits["some"] - logits["dense"]).abs().max() > 2 * tol
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("model,kv", [("tiny-qwen3", "bf16"), ("tiny-qwen2-d128", "fp8"), ("tiny-qwen2-d128", "q4")])
+def test_gpu_verify_graph_reads_selected_pages(model, kv, cuda_errors_clean):
+    """The captured verify step (a batch padded to its bucket, items shorter than the step)
+    against the eager one: every token has the eager logits' maximum within rounding, which
+    dense attention's logits do not bear out."""
+    from vramancer_b200.engine.runner import PrefillItem
+    llm = gpu_llm(model, kv, True, sparse_pages=4, enable_prefix_cache=False)
+    prompts = [PROMPTS[0], PROMPTS[0][5:] + [3] * 60, PROMPTS[1]]
+    tables = [list(range(32 * i, 32 * i + 20)) for i in range(3)]
+    pos = lambda i, a, b: [16 * tables[i][p // 16] + p % 16 for p in range(a, b)]  # noqa: E731
+    llm.runner.prefill([PrefillItem(p, 0, pos(i, 0, len(p)), tables[i], len(p), True) for i, p in enumerate(prompts)],
+                       [0.0] * 3, [0] * 3, [1.0] * 3, [0] * 3)
+    before = llm.pool.cache.clone(), llm.pool.key_bounds.clone()
+    feeds = [[5, 6, 7, 8, 9], [11], [2, 4, 2]]
+    items = [PrefillItem(f, len(p), pos(i, len(p), len(p) + len(f)), tables[i], len(p) + len(f), True)
+             for i, (p, f) in enumerate(zip(prompts, feeds))]
+
+    def restore():
+        llm.pool.cache.copy_(before[0])
+        llm.pool.key_bounds.copy_(before[1])
+
+    for _ in range(2):                                       # captured, then replayed
+        got = llm.runner.verify_greedy(items)
+        after = llm.pool.cache.clone(), llm.pool.key_bounds.clone()
+        restore()
+    assert [len(x) for x in got] == [5, 1, 3] and llm.runner._verify
+    eager = llm.runner.prefill_logits(items, decode_rows=True).float()
+    written = sum((it.slots for it in items), [])
+    rest = torch.ones(llm.pool.cache.shape[0], 16, dtype=torch.bool, device="cuda")
+    rest.view(-1)[torch.tensor(written, device="cuda")] = False
+    moved = (after[0].view(torch.uint8) != before[0].view(torch.uint8)).any(-1).any(1).any(1).any(1)
+    assert not (moved & rest).any()                          # padded rows store nothing
+    restore()
+    dense = llm.runner.prefill_logits(items).float()
+    # bf16 activations through two layers: a few units of 2^-8 of the logits' scale
+    tol = 8 * 2.0 ** -8 * eager.abs().max()
+    tok = torch.tensor(sum(got, []), device="cuda")[:, None]
+    assert (eager.gather(1, tok) >= eager.amax(1, keepdim=True) - tol).all()
+    assert (dense - eager).abs().max() > 2 * tol
+    assert (dense.gather(1, tok) < dense.amax(1, keepdim=True) - tol).any()
