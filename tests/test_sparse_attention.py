@@ -456,6 +456,37 @@ def test_select_extreme_values(dev, kind):
     assert got[3, 0].tolist() == list(range(15)) + [39]
 
 
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("kind", ["bf16", "fp8"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("pair", [False, True])
+@pytest.mark.parametrize("j", [6, 8, 10, 12, 14, 18, 23])
+def test_select_beside_cancelling_terms(dev, kind, D, pair, j):
+    """One term of every 16 dims is 1 (with `pair` another is -1), the others are 2^-j and
+    less, all of one sign: sums that drop low places of the small terms are off alike in all
+    pages or not, by up to the selection's error bound.  64-bit sums are exact."""
+    Hq, n, budget = 1, 900, 300
+    g = torch.Generator().manual_seed(100 * j + D)
+    steps = 16 if kind == "fp8" else 128
+    kb = torch.randint(steps // 2, steps + 1, (n, 1, 1, 2, D), generator=g).float() / steps
+    kb = kb.sort(3).values                                    # minima, maxima
+    q = torch.randint(64, 128, (1, D), generator=g).float() / 128 * 2.0 ** -j
+    q[0, ::16] = 1.0
+    kb[..., ::16] = 1.0
+    if pair:
+        q[0, 1::16] = -1.0
+        kb[..., 1::16] = 1.0
+    # half of the pages: small terms in two of three dims only
+    kb[::2, :, :, :, 2::3] = torch.where(torch.arange(2, D, 3) % 16 < 2, kb[::2, :, :, :, 2::3], 0.0)
+    dt = torch.float8_e4m3fn if kind == "fp8" else torch.bfloat16
+    assert torch.equal(kb.to(dt).float(), kb) and torch.equal(q.bfloat16().float(), q)
+    bt = torch.randperm(n, generator=g).int()[None]
+    kb, q = kb.to(dt).to(dev), q.bfloat16().to(dev)
+    got = ops.select_pages(q, kb, 0, bt.to(dev), i32([16 * n - 7], dev), Hq, budget, sinks=1, recent=1).cpu()
+    want = select_ref(q, kb, 0, bt, {0: (0, 16 * n - 7)}, Hq, budget, 1, 1)
+    assert got[0, 0].tolist() == want[0, 0]
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["bf16", "fp8"])
 @pytest.mark.parametrize("rows,n", [(1, 6001), (3, 2999), (40, 1201)])
