@@ -265,6 +265,29 @@ def test_append_rising_slots_with_gaps(dev):
     assert kb[0, 0, 0, :, 0].tolist() == [-4.0, 0.0]
 
 
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("kind", ["bf16", "fp8", "q4"])
+@pytest.mark.parametrize("scale", [1.0, 2.0 ** -9, 300.0])
+def test_bounds_hold_for_every_key(dev, kind, scale):
+    """No stored key gives a group a larger sum of scores than its page's bounds do; bounds of
+    four-bit keys, which are rounded to bf16, may fall short by half a step of each."""
+    Hq, KH, D, n = 8, 2, 64, 71
+    g = torch.Generator().manual_seed(int(scale))
+    cache, ks = make_pool(kind, 6, 1, KH, D, dev)
+    kb = ops.key_bounds_for(cache)
+    qkv = (torch.randn(n, (Hq + 2 * KH) * D, generator=g) * scale).bfloat16().to(dev)
+    q = ops.qk_norm_rope_kv_write(qkv, None, None, 0.0, None, None, cache, i32(list(range(16, 16 + n)), dev), ks, 0,
+                                  Hq, KH, D, key_bounds=kb).cpu().double().view(n, KH, -1, D)
+    keys = values(cache)[1:, 0, 0].transpose(0, 1).reshape(KH, -1, D)[:, :n]            # before kv_scale
+    b = kb.cpu().float().double()[1:, 0].repeat_interleave(16, 0)[:n].transpose(0, 1)   # [KH, token, 2, D]
+    up, dn = q.clamp(min=0).sum(2).transpose(0, 1), q.clamp(max=0).sum(2).transpose(0, 1)
+    score = torch.einsum("hqd,hkd->hqk", up, b[:, :, 1]) + torch.einsum("hqd,hkd->hqk", dn, b[:, :, 0])
+    exact = torch.einsum("hqd,hkd->hqk", q.sum(2).transpose(0, 1), keys)
+    mag = torch.einsum("hqd,hkd->hqk", up, b[:, :, 1].abs()) - torch.einsum("hqd,hkd->hqk", dn, b[:, :, 0].abs())
+    slack = U[torch.bfloat16] * (1 + 2.0 ** -7) if kind == "q4" else 0.0                # of the key, by its bound
+    assert (exact <= score + (slack + 2.0 ** -45) * mag).all()
+
+
 # ---------------------------------------------------------------------------- selection
 def rows_of(T, ctx, cu):
     if cu is None:

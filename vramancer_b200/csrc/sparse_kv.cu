@@ -593,7 +593,8 @@ void qk_norm_rope_kv_write(const AppendArgs& in, cudaStream_t st) {
 // ================================================================ page selection
 // Score of page p for the group's heads g:  sum_d (up_d * max_pd + dn_d * min_pd) with
 // up_d = sum_g max(q_gd, 0), dn_d = sum_g min(q_gd, 0): no key of the page gives the group
-// a larger sum of scores.
+// a larger sum of scores (four-bit keys: by more than the bounds' rounding to the nearest
+// bf16, 2^-8 sum_d (|up_d max_pd| + |dn_d min_pd|)).
 //
 // Which page is the last to be taken depends on differences of any size, so the choice is
 // the one that 64-bit sums make (products of 8-bit significands are exact there), ties to
@@ -608,8 +609,9 @@ void qk_norm_rope_kv_write(const AppendArgs& in, cudaStream_t st) {
 // scored again in 64 bits.  How an MMA rounds its sum is not documented: 2^-23 a term is an
 // assumption, that it keeps at least the 24 places of fp32 below its largest term.  Measured on
 // B200 against exact sums (32 products, exponents up to 20 apart, one term or a cancelling pair
-// above 31 terms that lose their last places): at most 8.9 * 2^-23 bf16, 7.9 * 2^-23 f16.  Whatever fp32 cannot decide (S out of range, non-finite values, more pages
-// between than kSelList) is decided by 64-bit scores of all pages.
+// above 31 terms that lose their last places): at most 8.9 * 2^-23 bf16, 7.9 * 2^-23 f16.
+// Whatever fp32 cannot decide (S out of range, non-finite values, more pages between than
+// kSelList) is decided by 64-bit scores of all pages.
 //
 // Bound by the reads while pages stream (64 rows of 32k tokens, fp8 bounds: 56.4 us, 4.8 TB/s;
 // 23k tokens, bf16: 58.1 us, 5.1 TB/s), but a row's start and choice (about 15k cycles of

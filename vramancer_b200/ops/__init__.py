@@ -464,7 +464,8 @@ def qk_norm_rope_kv_write(qkv: torch.Tensor, wq: Optional[torch.Tensor], wk: Opt
 
     With `key_bounds` (`key_bounds_for`) every page that is written gets the elementwise
     minimum and maximum of its stored keys, from its first row to the last row written here
-    (rows behind are not part of the sequence).  For that the tokens of a page must be
+    (rows behind are not part of the sequence): exactly for bf16 and fp8 pages, rounded to the
+    nearest bf16 for four-bit ones.  For that the tokens of a page must be
     adjacent in the batch, in rising slots, as the tokens of a prefill chunk, a verify step
     and a decode batch are.  Infinite keys count as the largest finite value of
     the bounds' type, a NaN as both its extremes.  Slots must be distinct; a slot < 0 is not
@@ -566,7 +567,9 @@ def select_pages(q: torch.Tensor, key_bounds: torch.Tensor, layer: int, block_ta
         sum_d ( sum_g max(q_gd, 0) * max_d  +  sum_g min(q_gd, 0) * min_d ),
 
     g over the query heads of the kv head: no key of the page gives the group a larger sum of
-    scores (key_bounds hold min <= max, as the append leaves them).  Scores are compared in
+    scores (key_bounds hold min <= max, as the append leaves them).  Where bounds are rounded
+    keys (four-bit pages, and fp32 pools on the CPU: to the nearest bf16), a key's sum may be
+    larger by 2^-8 of the terms' magnitudes.  Scores are compared in
     64 bits; ties go to the lowest page, a NaN comes first.  Block tables have at most
     SELECT_MAX_PAGES columns."""
     if q.is_cuda:
