@@ -945,6 +945,33 @@ def test_offsets_beyond_32_bits(cuda_errors_clean):
     assert all(torch.equal(x, y) for x, y in zip(*res))
 
 
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("kind", ["bf16", "fp8", "q4"])
+def test_nothing_to_do(dev, kind):
+    """No tokens, block tables without columns, lists without entries."""
+    KH, D = 2, 64
+    cache, ks = make_pool(kind, 3, 1, KH, D, dev)
+    kb, before = ops.key_bounds_for(cache), cache.clone()
+    none, two = i32([], dev), i32([0, 0], dev)
+    q = ops.qk_norm_rope_kv_write(torch.zeros(0, 8 * D).bfloat16().to(dev), None, None, 0.0, None, None, cache, none, ks,
+                                  0, 4, KH, D, key_bounds=kb)
+    assert q.shape == (0, 4 * D) and torch.equal(cache.view(torch.uint8), before.view(torch.uint8))
+    empty = torch.zeros(0, 2, dtype=torch.int32, device=dev)
+    p = ops.select_pages(q, kb, 0, empty, none, 4, 3)
+    assert p.shape == (0, KH, 3)
+    assert ops.paged_attention_selected(q, cache, 0, empty, none, p, ks, 1.0, 4).shape == (0, 4 * D)
+    q = torch.ones(2, 4 * D).bfloat16().to(dev)
+    flat = torch.zeros(2, 0, dtype=torch.int32, device=dev)
+    for ctx in (two, i32([40, 7], dev)):
+        p = ops.select_pages(q, kb, 0, flat, ctx, 4, 3)
+        assert (p == -1).all() and p.shape == (2, KH, 3)
+        o = ops.paged_attention_selected(q, cache, 0, flat, ctx, p, ks, 1.0, 4)
+        assert o.shape == (2, 4 * D) and (o == 0).all()
+        o = ops.paged_attention_selected(q, cache, 0, torch.zeros(2, 3, dtype=torch.int32, device=dev), ctx,
+                                         p[:, :, :0].contiguous(), ks, 1.0, 4)
+        assert (o == 0).all()
+
+
 # ---------------------------------------------------------------------------- refusals
 def test_refusals_cpu():
     q = torch.zeros(1, 128).bfloat16()
