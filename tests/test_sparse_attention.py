@@ -987,6 +987,20 @@ def test_refusals_cpu():
                                   ctx, None, 0, 2, 1, 32)
 
 
+@pytest.mark.parametrize("dev", DEVICES)
+def test_budgets_near_the_32_bit_limit_are_refused(dev):
+    """The kernel's indexes run a little past the budget and the sinks: they must not wrap."""
+    q = torch.zeros(1, 128).bfloat16().to(dev)
+    kb = torch.zeros(4, 1, 1, 2, 64).bfloat16().to(dev)
+    bt, ctx = i32([[0, 1, 2, 3]], dev), i32([64], dev)
+    for bad in (dict(budget=2 ** 30 + 1), dict(budget=2 ** 31 - 1), dict(budget=2 ** 31 - 1, sinks=2 ** 31 - 100),
+                dict(budget=2 ** 31), dict(budget=2 ** 40, sinks=2 ** 40 - 9)):
+        with pytest.raises((ValueError, RuntimeError)):
+            ops.select_pages(q, kb, 0, bt, ctx, 2, **bad)
+    got = ops.select_pages(q, kb, 0, bt, ctx, 2, 100000, sinks=99999)
+    assert got[0, 0, :4].tolist() == [0, 1, 2, 3] and (got[0, 0, 4:] == -1).all()
+
+
 @pytest.mark.gpu
 def test_refusals(cuda_errors_clean):
     dev = "cuda"

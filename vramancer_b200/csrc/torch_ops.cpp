@@ -532,8 +532,9 @@ Tensor select_pages(const Tensor& q, const Tensor& key_bounds, int64_t layer, co
   const char* op = "select_pages";
   check_bounds(key_bounds, op);
   TORCH_CHECK(layer >= 0 && layer < key_bounds.size(1), op, ": layer out of range");
-  TORCH_CHECK(sinks >= 0 && recent >= 1 && budget >= sinks + recent && budget <= INT32_MAX, op,
-              ": needs sinks >= 0, recent >= 1 and budget >= sinks + recent");
+  // 2^30: a warp's indexes run past sinks and budget by a few thousand and stay 32-bit
+  TORCH_CHECK(sinks >= 0 && recent >= 1 && budget >= sinks + recent && budget <= (1 << 30), op,
+              ": needs sinks >= 0, recent >= 1, budget >= sinks + recent and budget <= 2^30");
   vrm::SelectArgs a;
   set_rows(a, q, block_tables, context_lens, cu_q, Hq, key_bounds.size(2), key_bounds.size(4), op);
   same_device(q, {&key_bounds}, op);

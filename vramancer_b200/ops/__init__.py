@@ -577,8 +577,8 @@ def select_pages(q: torch.Tensor, key_bounds: torch.Tensor, layer: int, block_ta
                                      recent, cu_q, out)
     if block_tables.shape[1] > SELECT_MAX_PAGES:
         raise ValueError(f"select_pages: more than {SELECT_MAX_PAGES} pages a sequence")
-    if sinks < 0 or recent < 1 or budget < sinks + recent:
-        raise ValueError("select_pages: needs sinks >= 0, recent >= 1 and budget >= sinks + recent")
+    if sinks < 0 or recent < 1 or budget < sinks + recent or budget > 2 ** 30:
+        raise ValueError("select_pages: needs sinks >= 0, recent >= 1, budget >= sinks + recent and budget <= 2^30")
     T = q.shape[0]
     KH, D = key_bounds.shape[2], key_bounds.shape[4]
     G = num_q_heads // KH
