@@ -1001,6 +1001,35 @@ def test_budgets_near_the_32_bit_limit_are_refused(dev):
     assert got[0, 0, :4].tolist() == [0, 1, 2, 3] and (got[0, 0, 4:] == -1).all()
 
 
+@pytest.mark.parametrize("dev", DEVICES)
+def test_lists_near_the_32_bit_limit_are_refused(dev):
+    q, cache = torch.zeros(1, 64).bfloat16().to(dev), torch.zeros(2, 1, 2, 1, 16, 64).bfloat16().to(dev)
+    bt, ctx = i32([[0, 1]], dev), i32([20], dev)
+    for n in (2 ** 30 + 1, 2 ** 31 - 1, 2 ** 31 + 5):
+        pages = torch.empty(1, 1, n, dtype=torch.int32, device=dev)          # not touched
+        with pytest.raises((ValueError, RuntimeError)):
+            ops.paged_attention_selected(q, cache, 0, bt, ctx, pages, None, 1.0, 1)
+        del pages
+
+
+@pytest.mark.gpu
+def test_block_table_rows_far_apart_are_refused(cuda_errors_clean):
+    """The distance of two rows of the table has to fit the kernels' 32 bits."""
+    q, kb = torch.zeros(2, 64, device="cuda").bfloat16(), torch.zeros(4, 1, 1, 2, 64, device="cuda").bfloat16()
+    cache, ctx = torch.zeros(4, 1, 2, 1, 16, 64, device="cuda").bfloat16(), i32([50, 50], "cuda")
+    store = torch.empty(2 ** 31 + 8, dtype=torch.int32, device="cuda")
+    far = store.as_strided((2, 4), (2 ** 31, 1))
+    far.copy_(i32([[0, 1, 2, 3], [3, 2, 1, 0]], "cuda"))
+    pages = i32([[[0, 1]], [[0, 3]]], "cuda")
+    with pytest.raises(RuntimeError):
+        ops.select_pages(q, kb, 0, far, ctx, 1, 2)
+    with pytest.raises(RuntimeError):
+        ops.paged_attention_selected(q, cache, 0, far, ctx, pages, None, 1.0, 1)
+    one = far[1:]                                             # a single row has no distance
+    assert ops.select_pages(q[:1], kb, 0, one, ctx[:1], 1, 2).tolist() == [[[0, 3]]]
+    assert (ops.paged_attention_selected(q[:1], cache, 0, one, ctx[:1], pages[:1], None, 1.0, 1) == 0).all()
+
+
 @pytest.mark.gpu
 def test_refusals(cuda_errors_clean):
     dev = "cuda"

@@ -500,8 +500,9 @@ void set_rows(Args& a, const Tensor& q, const Tensor& block_tables, const Tensor
   TORCH_CHECK(KH >= 1 && Hq >= 1 && Hq % KH == 0 && Hq / KH <= 8, op, ": GQA group must be <= 8 heads");
   TORCH_CHECK(D == 64 || D == 128, op, ": head_dim must be 64 or 128");
   TORCH_CHECK(q.size(1) >= Hq * D, op, ": q must be [T, >= Hq * D]");
-  TORCH_CHECK(block_tables.scalar_type() == torch::kInt32 && block_tables.dim() == 2 && block_tables.stride(1) == 1,
-              op, ": block_tables must be int32 [B, max_pages]");
+  TORCH_CHECK(block_tables.scalar_type() == torch::kInt32 && block_tables.dim() == 2 && block_tables.stride(1) == 1 &&
+                  block_tables.size(1) <= INT32_MAX && (block_tables.size(0) <= 1 || block_tables.stride(0) <= INT32_MAX),
+              op, ": block_tables must be int32 [B, max_pages], rows at most 2^31 - 1 entries apart");
   TORCH_CHECK(context_lens.scalar_type() == torch::kInt32 && context_lens.is_contiguous(), op, ": int32 context_lens");
   same_device(q, {&block_tables, &context_lens}, op);
   same_device_opt(q, {&cu_q}, op);
@@ -568,8 +569,8 @@ Tensor attn_selected(const Tensor& q, const Tensor& cache, int64_t layer, const 
   vrm::AttendArgs a;
   set_rows(a, q, block_tables, context_lens, cu_q, Hq, cache.size(3), cache_head_dim(cache), op);
   TORCH_CHECK(pages.scalar_type() == torch::kInt32 && pages.is_contiguous() && pages.dim() == 3 &&
-                  pages.size(0) >= q.size(0) && pages.size(1) == a.KH,
-              op, ": pages must be contiguous int32 [T, kv_heads, n]");
+                  pages.size(0) >= q.size(0) && pages.size(1) == a.KH && pages.size(2) <= (1 << 30),
+              op, ": pages must be contiguous int32 [T, kv_heads, n], n <= 2^30");
   same_device(q, {&cache, &pages}, op);
   same_device_opt(q, {&kv_scale, &out}, op);
   a.fmt = page_format(cache);

@@ -620,6 +620,8 @@ def paged_attention_selected(q: torch.Tensor, cache: torch.Tensor, layer: int, b
     if q.is_cuda:
         return native().paged_attention_selected(q, cache, layer, block_tables, context_lens, pages, kv_scale,
                                                  sm_scale, num_q_heads, cu_q, out)
+    if pages.shape[2] > 2 ** 30:
+        raise ValueError("paged_attention_selected: more than 2^30 list entries")
     T = q.shape[0]
     D = cache_head_dim(cache)
     KH = cache.shape[3]
