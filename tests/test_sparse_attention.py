@@ -771,6 +771,44 @@ def test_attend_non_finite_queries(dev, kind, bad, n_sel):
                 assert ((got[3 * h + i] - o[i]).abs() <= tol[i] * (1 + 2.0 ** -10)).all(), (h, i)
 
 
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("kind", ["bf16", "fp8", "q4"])
+@pytest.mark.parametrize("below", [12.0, 25.4, 30.0])
+@pytest.mark.parametrize("pages", [2, 700])
+def test_attend_many_small_weights(dev, kind, below, pages):
+    """One token 2^below above all others, which alone have values: their weights add up,
+    however small each is."""
+    x = torch.zeros(pages, 1, 2, 1, 16, 64)
+    x[0, 0, 0, 0, 3, 0] = 1.0                                 # the key that stands out, its value 0
+    x[:, 0, 1] = 1.0
+    x[0, 0, 1, 0, 3] = 0.0
+    dt = POOLS[kind]
+    cache, ks = q4.quantize(x) if kind == "q4" else x.to(dt), torch.ones(1, 2, 1) if kind == "fp8" else None
+    q = torch.zeros(1, 128)
+    q[0, 0], q[0, 64] = 1.0, 0.5
+    q = q.bfloat16()
+    bt, lst = torch.arange(pages, dtype=torch.int32)[None], torch.arange(pages, dtype=torch.int32)[None, None]
+    sm = below * math.log(2)
+    got = ops.paged_attention_selected(q.to(dev), cache.to(dev), 0, bt.to(dev), i32([16 * pages], dev), lst.to(dev),
+                                       None if ks is None else ks.to(dev), sm, 2).cpu().double().view(2, 64)
+    vals = values(cache, ks)[:, 0]
+    k, v = vals[:, 0, 0].flatten(0, 1), vals[:, 1, 0].flatten(0, 1)
+    s = q.double().view(2, 64) @ k.t() * sm
+    w = torch.softmax(s, -1)
+    o = w @ v
+    # output rounding; each weight's (half a step, in f16 at least 2^-39 of the largest); fp32
+    # scores, 2^-18 of their size, above and below the fraction
+    half = U[torch.bfloat16] if kind == "bf16" else U[torch.float16]
+    small = 0 if kind == "bf16" else 2.0 ** -39 * w.amax(-1, keepdim=True) * 16 * pages
+    tol = (U[torch.bfloat16] + half + 2.0 ** -17 * s.abs().amax(-1, keepdim=True) + 2.0 ** -18) * o + small
+    if kind == "q4":
+        # keys and values become f16: the stored key, 15 * f16(1 / 15) = 1 - 2^-12, lies half a
+        # step of f16 from its neighbours.  Scores move by up to 2^-11 of themselves, weights
+        # and their sum by that much each; values by 2^-11
+        tol = tol + (2 * U[torch.float16] * s.abs().amax(-1, keepdim=True) + U[torch.float16]) * o
+    assert ((got - o).abs() <= tol).all(), (float(got[0, 0]), float(o[0, 0]))
+
+
 # ---------------------------------------------------------------------------- as they are used
 @pytest.mark.parametrize("dev", DEVICES)
 @pytest.mark.parametrize("kind", ["bf16", "fp8", "q4"])

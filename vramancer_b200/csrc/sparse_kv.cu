@@ -1446,6 +1446,12 @@ __global__ void __launch_bounds__(128, AttendShape<D, FMT>::kCtas) attend_kernel
     k_scale = P.kv_scale[(P.layer * 2 + 0) * KH + kvh];
     v_scale = P.kv_scale[(P.layer * 2 + 1) * KH + kvh];
   }
+  // Weights are rounded to the type of V's operands before their product: bf16 over bf16 pages
+  // (2^-8 of each), f16 over the others (2^-11), there times 2^14, so that a weight stays whole
+  // down to 2^-28 of the largest and counts down to 2^-39.  The sums that divide them are fp32
+  // sums of the weights before that rounding.
+  constexpr float kWeight = FMT == kFmtBf16 ? 1.f : 16384.f;
+  v_scale *= 1.f / kWeight;
   const float sm_log2 = P.sm_scale * 1.4426950408889634f;
   float scale_log2[2] = {sm_log2 * k_scale, sm_log2 * k_scale};
   RowOf row;
@@ -1586,8 +1592,8 @@ __global__ void __launch_bounds__(128, AttendShape<D, FMT>::kCtas) attend_kernel
           pb0 = transpose8x8(pack_bf16x2(x[q][0], x[q][1]));
           pb1 = transpose8x8(pack_bf16x2(x[q][2], x[q][3]));
         } else {
-          pb0 = transpose8x8(pack_half2(x[q][0], x[q][1]));
-          pb1 = transpose8x8(pack_half2(x[q][2], x[q][3]));
+          pb0 = transpose8x8(pack_half2(x[q][0] * kWeight, x[q][1] * kWeight));
+          pb1 = transpose8x8(pack_half2(x[q][2] * kWeight, x[q][3] * kWeight));
         }
 #pragma unroll
         for (int e = 0; e < kSteps; ++e) {
