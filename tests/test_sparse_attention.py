@@ -809,6 +809,36 @@ def test_attend_many_small_weights(dev, kind, below, pages):
     assert ((got - o).abs() <= tol).all(), (float(got[0, 0]), float(o[0, 0]))
 
 
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("n_sel,ctx", [(1, 5), (3, 48), (40, 633), (128, 2049)])
+def test_attend_weights_are_not_cut_to_bf16(dev, D, n_sel, ctx):
+    """Over bf16 pages only the output is rounded to eight bits: weights keep 16 (2^-16 of
+    each), scores and sums are fp32."""
+    Hq, KH, n = 8, 2, -(-ctx // 16)
+    cache, _ = make_pool("bf16", n, 1, KH, D, dev, seed=D + ctx)
+    q = torch.randn(2, Hq * D, generator=torch.Generator().manual_seed(ctx)).bfloat16().to(dev)
+    bt = torch.arange(n, dtype=torch.int32, device=dev).repeat(2, 1)
+    rows = {0: (0, ctx), 1: (1, max(1, ctx - 9))}
+    pages = choose_pages(rows, KH, 2, n_sel, 1, dev)
+    sm = 1 / math.sqrt(D)
+    got = ops.paged_attention_selected(q, cache, 0, bt, i32([n for _, n in rows.values()], dev), pages, None, sm, Hq)
+    got, vals, G = got.cpu().double(), values(cache)[:, 0], Hq // KH
+    for t, (b, m) in rows.items():
+        for h in range(KH):
+            sel = [p for p in pages[t, h].tolist() if p >= 0]
+            tok = torch.tensor([16 * p + o for p in sel for o in range(16) if 16 * p + o < m])
+            k, v = (vals[:, i, h].flatten(0, 1)[tok] for i in (0, 1))
+            qd = q[t, h * G * D:(h + 1) * G * D].cpu().double().view(G, D)
+            w = torch.softmax(qd @ k.t() * sm, -1)
+            worst = (qd.abs() @ k.abs().t() * sm).amax(-1, keepdim=True)
+            o, a = w @ v, w @ v.abs()
+            # fp32 scores: 2^-18 of their magnitudes' sum, above and below the fraction; fp32 sums
+            tol = U[torch.bfloat16] * o.abs() + (2.0 ** -16 + 2.0 ** -17 * worst + 2.0 ** -18) * a
+            e = (got[t, h * G * D:(h + 1) * G * D].view(G, D) - o).abs()
+            assert (e <= tol * (1 + 2.0 ** -10)).all(), (t, h, float((e / tol).max()))
+
+
 # ---------------------------------------------------------------------------- as they are used
 @pytest.mark.parametrize("dev", DEVICES)
 @pytest.mark.parametrize("kind", ["bf16", "fp8", "q4"])

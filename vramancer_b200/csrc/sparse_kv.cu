@@ -1446,10 +1446,12 @@ __global__ void __launch_bounds__(128, AttendShape<D, FMT>::kCtas) attend_kernel
     k_scale = P.kv_scale[(P.layer * 2 + 0) * KH + kvh];
     v_scale = P.kv_scale[(P.layer * 2 + 1) * KH + kvh];
   }
-  // Weights are rounded to the type of V's operands before their product: bf16 over bf16 pages
-  // (2^-8 of each), f16 over the others (2^-11), there times 2^14, so that a weight stays whole
-  // down to 2^-28 of the largest and counts down to 2^-39.  The sums that divide them are fp32
-  // sums of the weights before that rounding.
+  // Weights become operands beside V, of its type: bf16 over bf16 pages, in two parts that hold
+  // 16 bits of them (with one part outputs were off by 1.9e-3 of their norm instead of 1.7e-3, a
+  // bf16 result's own rounding; 32 rows of 128 pages 43.65 -> 43.9 us); f16 over the others, 11
+  // bits, which shows in no output's error (1.7e-3 either way).  The latter times 2^14, so that a
+  // weight stays whole down to 2^-28 of the largest and counts down to 2^-39.  The sums that
+  // divide them are fp32 sums of the weights before that rounding.
   constexpr float kWeight = FMT == kFmtBf16 ? 1.f : 16384.f;
   v_scale *= 1.f / kWeight;
   const float sm_log2 = P.sm_scale * 1.4426950408889634f;
@@ -1587,10 +1589,13 @@ __global__ void __launch_bounds__(128, AttendShape<D, FMT>::kCtas) attend_kernel
       }
 #pragma unroll
       for (int q = 0; q < kTurn; ++q) {
-        uint32_t pb0, pb1;
+        uint32_t pb0, pb1, pl0 = 0, pl1 = 0;                 // weights; bf16: and what they leave
         if constexpr (FMT == kFmtBf16) {
-          pb0 = transpose8x8(pack_bf16x2(x[q][0], x[q][1]));
-          pb1 = transpose8x8(pack_bf16x2(x[q][2], x[q][3]));
+          const uint32_t h0 = pack_bf16x2(x[q][0], x[q][1]), h1 = pack_bf16x2(x[q][2], x[q][3]);
+          pb0 = transpose8x8(h0);
+          pb1 = transpose8x8(h1);
+          pl0 = transpose8x8(pack_bf16x2(x[q][0] - bf16_lo(h0), x[q][1] - bf16_hi(h0)));
+          pl1 = transpose8x8(pack_bf16x2(x[q][2] - bf16_lo(h1), x[q][3] - bf16_hi(h1)));
         } else {
           pb0 = transpose8x8(pack_half2(x[q][0] * kWeight, x[q][1] * kWeight));
           pb1 = transpose8x8(pack_half2(x[q][2] * kWeight, x[q][3] * kWeight));
@@ -1599,8 +1604,12 @@ __global__ void __launch_bounds__(128, AttendShape<D, FMT>::kCtas) attend_kernel
         for (int e = 0; e < kSteps; ++e) {
           uint32_t a[4];
           f[q].v_frag(e, a);
-          if constexpr (FMT == kFmtBf16) mma_bf16_16816(o[e], a[0], a[1], a[2], a[3], pb0, pb1);
-          else mma_f16(o[e], a[0], a[1], a[2], a[3], pb0, pb1);
+          if constexpr (FMT == kFmtBf16) {
+            mma_bf16_16816(o[e], a[0], a[1], a[2], a[3], pb0, pb1);
+            mma_bf16_16816(o[e], a[0], a[1], a[2], a[3], pl0, pl1);
+          } else {
+            mma_f16(o[e], a[0], a[1], a[2], a[3], pb0, pb1);
+          }
         }
         if (more) f[q].load_v(kp[q] + (size_t)KH * head_b, r[q], g, c);
       }
