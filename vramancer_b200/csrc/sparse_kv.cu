@@ -112,7 +112,9 @@ __device__ __forceinline__ bool find_row(int t, const int* cu_q, const int* cont
 //
 // Bound by memory for prompts (8192 tokens, 32 + 4 heads: 30.2 us, 5.7 TB/s; with 2 or 8 heads'
 // rows in flight a lane instead of 4 35.1 and 35.2 us), by the chain of dependent loads for
-// decode steps (1 row 2.9 us, 64 rows of fp8 pages 4.5 us).
+// decode steps (1 row 2.9 us, 64 rows of fp8 pages 4.5 us).  Slower forms, 32 + 8 heads: 8192
+// tokens with a rotation of half the head 96.7 us (whole head 39.5: each pair passes through
+// shared memory), four-bit pages 50.1 (1 row 6.8, 64 rows 10.9: two divisions a value).
 template <int D>
 struct AppendShape {
   static constexpr int kLanes = D / 16;            // lanes of a row
@@ -552,8 +554,13 @@ __global__ void __launch_bounds__(128) append_kernel(AppendArgs a) {
 template <int D, int FMT>
 static void launch_append(AppendArgs a, cudaStream_t st) {
   // heads of a q or v block: the rotation table's row is read once a block, so as many as
-  // leave a block to every SM (B200, 32 + 8 heads, us with 4 / 8 / 16 heads a block: 512 tokens
-  // 5.0 / 6.7 / 9.2, 2048 tokens 14.6 / 13.1 / 12.9; 8192 tokens with all 32: 30.0, with 4: 32.5)
+  // leave a block to every SM.  B200, us with 4 / 8 / 16 / 32 heads a block, this rule's choice
+  // in brackets, 32 + 8 heads: 512 tokens (4.5) / 5.5 / 8.4 / 12.8, 2048: 12.1 / 10.9 / (12.9) /
+  // 20.2, 2400: 13.8 / 12.4 / 13.0 / (22.9), 3251: 17.3 / 16.4 / 15.3 / (21.5), 4096: 22.1 /
+  // 20.7 / 19.8 / (22.7), 6144: 32.1 / 30.9 / 30.7 / (28.8), 8192: 42.1 / 41.3 / 40.7 / (39.5).
+  // It suits decode steps and long prompts.  From one block an SM (2353 tokens of 128 dims) to
+  // about 5000 tokens 8 or 16 heads are faster, by up to 1.8 times (40 + 8 heads: 2.1): there
+  // one block an SM is too few.
   const int tiles = (a.T + AppendShape<D>::kRows - 1) / AppendShape<D>::kRows;
   int per = 4;
   while (per < a.Hq && (long long)tiles * ((a.Hq + 2 * per - 1) / (2 * per)) >= device_sm_count()) per *= 2;
@@ -649,7 +656,10 @@ __device__ __forceinline__ float from_sortable(uint32_t k) { return __uint_as_fl
 
 // Pages decided by the short 64-bit path.  An outlier channel makes E large beside the spread
 // of the scores: with 32 and one channel 400 times the others, 64 rows of 2048 pages of fp8
-// bounds took 471 us instead of 73, 1 row of 24576 pages 1105 instead of 43.
+// bounds took 471 us instead of 73, 1 row of 24576 pages 1105 instead of 43.  Beyond 128 pages
+// all candidates are scored in 64 bits, by one CTA: with bf16 bounds and one channel 4000 times
+// the others 1 row of 2048 pages takes 90 us (8 times: 10), of 24576 pages 1235 (86), 64 rows of
+// 2048 pages 489 (92).  A key that was infinite, and so has the largest bound, does the same.
 constexpr int kSelList = 128;
 constexpr int kSelMaxPages = 24576;              // candidate pages of a row (8 bytes of shared memory each)
 constexpr int kBins = 1024;
@@ -1205,6 +1215,10 @@ __global__ void __launch_bounds__(NT, 512 / NT) select_kernel(SelectArgs a) {
 
 template <int D, bool F8, int NT>
 static void launch_select(const SelectArgs& a, int nc, cudaStream_t st) {
+  // by the table's width, not the contexts': where it leaves an SM fewer CTAs, short contexts
+  // are slower too.  B200, us, 16000 tokens with tables of 1000 / 4096 / 6144 / 8192 / 12288 /
+  // 24576 columns: 64 rows (bf16) 49.7 / 60.9 / 79.8 / 148 / 112 / 131, 32 rows 27.9 / 28.1 /
+  // 28.0 / 29.0 / 56.2 / 62.0; 1 row of 32000 tokens 9.9 up to 16384 columns, 10.6 with 24576.
   const size_t smem = (size_t)a.max_pages * sizeof(uint64_t);
   auto kern = select_kernel<D, F8, NT>;
   if (smem > 32 * 1024)
@@ -1389,10 +1403,10 @@ struct Frag {
 }  // namespace
 
 // Pages a warp takes at a time and CTAs an SM holds.  Pages of 8 KB (bf16, D = 128): two
-// at a time in 244 registers, so that each of the SM's 8 warps has 16 KB under way; narrower
+// at a time in 255 registers, so that each of the SM's 8 warps has 16 KB under way; narrower
 // pages cost more arithmetic a byte, and 16 warps with one page each run better (B200, us:
 // 32 rows of bf16 43.9 against 77.9 with one page and 4 CTAs; 128 rows of fp8 92.0 against
-// 96.0 with four pages and 2 CTAs, four-bit 64 rows 58.1 against 59.4).
+// 97.0 with four pages and 2 CTAs, 128 four-bit rows 104.2 against 107.7).
 template <int D, int FMT>
 struct AttendShape {
   static constexpr bool kWide = FMT == kFmtBf16 && D == 128;
@@ -1718,7 +1732,7 @@ template <int D, int FMT>
 static void launch_attend(const AttendArgs& a, cudaStream_t st) {
   // as many splits as keep all CTAs resident at once and leave every warp two pages: more
   // CTAs than that queue, and each costs its start and its merge again (B200, us, splits
-  // 1 / 2 / 8: 1 row of bf16 25.0 / 16.4 / 8.7, 16 rows 35.9 / 26.1 / 46.8, 64 rows 83.8 / 99.6 / 156.7)
+  // 1 / 2 / 8: 1 row of bf16 25.1 / 15.6 / 7.6, 16 rows 34.9 / 25.6 / 39.6, 64 rows 84.4 / 96.9 / 139)
   int splits = 1;
   while (splits < 8 && (long long)a.T * a.KH * splits * 2 <= (long long)AttendShape<D, FMT>::kCtas * device_sm_count() &&
          a.S >= 16 * splits)

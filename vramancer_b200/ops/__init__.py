@@ -571,7 +571,8 @@ def select_pages(q: torch.Tensor, key_bounds: torch.Tensor, layer: int, block_ta
     keys (four-bit pages, and fp32 pools on the CPU: to the nearest bf16), a key's sum may be
     larger by 2^-8 of the terms' magnitudes.  Scores are compared in
     64 bits; ties go to the lowest page, a NaN comes first.  Block tables have at most
-    SELECT_MAX_PAGES columns."""
+    SELECT_MAX_PAGES columns; columns that no context reaches cost time too, so a table should
+    not be much wider than the contexts need."""
     if q.is_cuda:
         return native().select_pages(q, key_bounds, layer, block_tables, context_lens, num_q_heads, budget, sinks,
                                      recent, cu_q, out)
